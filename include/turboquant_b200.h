@@ -471,6 +471,83 @@ int tq_rows_scores(const tq_consts* consts, const uint8_t* codes, const uint8_t*
 int tq_pack_stage(const tq_consts* consts, const float* y, const float* projected, int64_t n_rows,
                   uint8_t* codes, uint8_t* signs, void* stream);
 
+/* ---- the exact paged cache -------------------------------------------------
+ *
+ * Keys and values as they are, bf16 or fp16, in pages of `block_size` tokens: what an engine holds for the layers that it does
+ * not compress, what tq_store_paged reads, and what is evicted from before it is compressed.  No counterpart in the reference,
+ * which leaves these to its engine.  None of the calls reads or writes a row outside the pages: an index that would lead there
+ * is skipped and reported in *status (a device word that the caller zeroed; the first error stays). */
+
+/* Element (block, token, head, :) of a plane is at base + block*stride_block + token*stride_token + head*stride_head (in
+ * elements, the same for both planes), head_dim contiguous; bases and strides 16-byte aligned.  head_dim 64, 128 or 256. */
+typedef struct tq_pages {
+    void* key;
+    void* value;
+    tq_dtype dtype;          /* TQ_BF16 or TQ_F16 */
+    int32_t block_size;      /* tokens per page, any number */
+    int64_t num_blocks;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int64_t stride_block, stride_token, stride_head;
+} tq_pages;
+
+/* The sequences of a call: logical block j of sequence b is at physical block block_tables[b*table_stride + j], j <
+ * table_width.  A length below 0 or above max_seq_len is clamped and reported. */
+typedef struct tq_pages_batch {
+    const int32_t* block_tables;   /* device */
+    int32_t table_stride, table_width;
+    const int32_t* seq_lens;       /* (batch), device */
+    int32_t batch;
+    int32_t max_seq_len;           /* host upper bound; table_width * block_size covers it */
+} tq_pages_batch;
+
+/* What the tokens of `batch` cached sequences have received, kv head by kv head; rows of `max_tokens`.  Slots below held[b] have
+ * the position noted in `positions`; the slots behind were filled after the last tq_pages_evict, in order, from position
+ * seen[b] on.  Before the first one held and seen are 0. */
+typedef struct tq_pages_ledger {
+    float* mass;          /* (batch, num_kv_heads, max_tokens): sum of the softmax weights received */
+    int32_t* positions;   /* (batch, num_kv_heads, max_tokens) */
+    int32_t* held;        /* (batch) */
+    int32_t* seen;        /* (batch) */
+    int32_t max_tokens;
+} tq_pages_ledger;
+
+/* Copy n_tokens key / value rows into the pages: token t to slot slot_mapping[t] = block*block_size + offset; a negative slot
+ * is a padding token.  Rows 16-byte aligned.  Slots are distinct: of two tokens with one slot either may stay, mixed even. */
+int tq_pages_write(const tq_pages* pages, const void* key, const void* value, int64_t n_tokens, int64_t key_stride_token,
+                   int64_t key_stride_head, int64_t value_stride_token, int64_t value_stride_head, const int64_t* slot_mapping,
+                   int32_t* status, void* stream);
+
+/* Bytes of the tickets of tq_pages_decode and tq_pages_observe: zeroed once, zero again after every call.  Calls that may run at
+ * the same time need tickets (and scratch, of any content) of their own. */
+size_t tq_pages_ticket_bytes(void);
+int tq_pages_decode_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t num_q_heads, int32_t with_mass, size_t* out);
+
+/* Attention of one new token per sequence, already in the pages as the last of its seq_lens tokens: query and out
+ * (batch, num_q_heads, head_dim) contiguous, in the pages' dtype; any number of query heads per kv head.  An empty sequence's
+ * output is zero.  With `mass` ((batch, num_kv_heads, mass_stride) fp32): the softmax weight of every cached token, summed over
+ * the kv head's query heads, is added to it. */
+int tq_pages_decode(const tq_pages* pages, const tq_pages_batch* batch, const void* query, int32_t num_q_heads, float scale, void* out,
+                    float* mass, int64_t mass_stride, void* scratch, size_t scratch_bytes, int32_t* tickets, int32_t* status,
+                    void* stream);
+
+/* The weights of the last `window` queries of every sequence alone: query (batch, window, num_q_heads, head_dim) contiguous, query
+ * i of a sequence of n tokens at position n - window + i, where it sees the tokens up to its own (one before the first token
+ * sees nothing); their softmax weights, summed over the window and the kv head's query heads, are added to `mass`. */
+int tq_pages_observe_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t window, int32_t num_q_heads, size_t* out);
+int tq_pages_observe(const tq_pages* pages, const tq_pages_batch* batch, const void* query, int32_t window, int32_t num_q_heads,
+                     float scale, float* mass, int64_t mass_stride, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+
+/* Bring every sequence down to `budget` tokens, kv head by kv head.  Of n > budget tokens the `recent` latest by position stay,
+ * then those with the largest mass (NaN above all numbers, ties: the lower slot).  Tokens kept in slots from `budget` on move,
+ * in ascending order, into the free slots before it: rows, mass and position; rows from `budget` on stay as they are.  `out`
+ * receives the ledger (mass 0 and position -1 behind the tokens that are left, up to max_tokens) and may be `ledger` itself;
+ * new_lens (batch) the lengths.  Sequences do not share pages. */
+int tq_pages_evict_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t budget, size_t* out);
+int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch, const tq_pages_ledger* ledger, const tq_pages_ledger* out,
+                   int32_t budget, int32_t recent, int32_t* new_lens, void* scratch, size_t scratch_bytes, int32_t* status,
+                   void* stream);
+
 /* Zero a workspace (status word and tickets must start at zero; kernels leave
  * them zero again).  Call once after allocating it. */
 int tq_workspace_init(void* workspace, size_t bytes, void* stream);

@@ -10,5 +10,6 @@ from .capture import RingBuffer, KVCaptureEngine
 from .store import CompressedKVStore
 from .score import compute_hybrid_attention
 from .paged_cache import CompressedCacheSpec, CompressedPagedKVCache
+from .exact_cache import AttentionLedger, ExactCacheSpec, PagedKVCache
 
 __version__ = "0.1.0"

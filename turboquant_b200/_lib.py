@@ -63,6 +63,22 @@ class tq_decode_args(C.Structure):
                 ("ring_capacity", C.c_int32), ("flags", C.c_int32)]
 
 
+class tq_pages(C.Structure):
+    _fields_ = [("key", C.c_void_p), ("value", C.c_void_p), ("dtype", C.c_int32), ("block_size", C.c_int32),
+                ("num_blocks", C.c_int64), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("stride_block", C.c_int64),
+                ("stride_token", C.c_int64), ("stride_head", C.c_int64)]
+
+
+class tq_pages_batch(C.Structure):
+    _fields_ = [("block_tables", C.c_void_p), ("table_stride", C.c_int32), ("table_width", C.c_int32), ("seq_lens", C.c_void_p),
+                ("batch", C.c_int32), ("max_seq_len", C.c_int32)]
+
+
+class tq_pages_ledger(C.Structure):
+    _fields_ = [("mass", C.c_void_p), ("positions", C.c_void_p), ("held", C.c_void_p), ("seen", C.c_void_p),
+                ("max_tokens", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/turboquant_b200.h declares
 SIGNATURES = {
     "tq_get_layout": (C.c_int, [C.POINTER(tq_config), C.POINTER(tq_layout)]),
@@ -134,6 +150,21 @@ SIGNATURES = {
                                  C.c_void_p]),
     "tq_pack_stage": (C.c_int, [C.POINTER(tq_consts), C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
                                 C.c_void_p]),
+    "tq_pages_write": (C.c_int, [C.POINTER(tq_pages), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                                 C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "tq_pages_ticket_bytes": (C.c_size_t, []),
+    "tq_pages_decode_scratch_bytes": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.c_int32, C.c_int32,
+                                                C.POINTER(C.c_size_t)]),
+    "tq_pages_decode": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.c_void_p, C.c_int32, C.c_float, C.c_void_p,
+                                  C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "tq_pages_observe_scratch_bytes": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.c_int32, C.c_int32,
+                                                 C.POINTER(C.c_size_t)]),
+    "tq_pages_observe": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.c_void_p, C.c_int32, C.c_int32, C.c_float,
+                                   C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "tq_pages_evict_scratch_bytes": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.c_int32, C.POINTER(C.c_size_t)]),
+    "tq_pages_evict": (C.c_int, [C.POINTER(tq_pages), C.POINTER(tq_pages_batch), C.POINTER(tq_pages_ledger),
+                                 C.POINTER(tq_pages_ledger), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+                                 C.c_void_p]),
     "tq_workspace_init": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
     "tq_read_status": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_int32)]),
 }

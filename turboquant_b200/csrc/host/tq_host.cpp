@@ -10,6 +10,7 @@
 // launched, and the Python wrapper goes its general way.  Status codes of the library come back as ints.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -513,7 +514,201 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ the exact paged cache
+
+// What every call on pages has: the pages' tensor (for the device), the status word, the sequences.  Scratch comes from torch's
+// allocator call by call, so that calls on several streams or in several captured graphs share nothing.
+struct PagesCall {
+    const tq_pages* pages = nullptr;
+    const at::Tensor* status = nullptr;
+    tq_pages_batch batch = {};
+};
+inline bool on(const at::Tensor& t, const at::Tensor& like) { return t.is_cuda() && t.get_device() == like.get_device(); }
+// pages, status, block tables, lengths and their bound; false: not as the kernels take them
+bool pages_call(PagesCall& c, PyObject* pages, PyObject* status, PyObject* tables, PyObject* lens, PyObject* max_len, int64_t batch) {
+    c.pages = address<const tq_pages>(pages);
+    c.status = tensor_or_null(status);
+    const at::Tensor *t = tensor_or_null(tables), *n = tensor_or_null(lens);
+    const int64_t longest = PyLong_AsLongLong(max_len);
+    if (PyErr_Occurred() || !c.status || !t || !n || longest < 1 || longest > INT32_MAX || batch < 1 || batch > INT32_MAX) return false;
+    if (!on(*t, *c.status) || !on(*n, *c.status) || t->dim() != 2 || t->scalar_type() != at::kInt || t->stride(1) != 1 || t->size(0) < batch ||
+        t->size(1) < 1 || t->size(1) > INT32_MAX || (t->size(0) > 1 && t->stride(0) < t->size(1)) || t->stride(0) > INT32_MAX || n->dim() != 1 ||
+        n->scalar_type() != at::kInt || n->size(0) < batch || !n->is_contiguous() || t->size(1) * c.pages->block_size < longest)
+        return false;
+    c.batch.block_tables = t->data_ptr<int32_t>();
+    c.batch.table_width = (int32_t)t->size(1);
+    c.batch.table_stride = t->size(0) > 1 ? (int32_t)t->stride(0) : c.batch.table_width;
+    c.batch.seq_lens = n->data_ptr<int32_t>();
+    c.batch.batch = (int32_t)batch;
+    c.batch.max_seq_len = (int32_t)longest;
+    return true;
+}
+// a row per sequence and kv head, `type`, contiguous, long enough
+inline bool plane_ok(const at::Tensor* t, const PagesCall& c, at::ScalarType type) {
+    return t && on(*t, *c.status) && t->dim() == 3 && t->is_contiguous() && t->scalar_type() == type && t->size(0) >= c.batch.batch &&
+           t->size(1) == c.pages->num_kv_heads && t->size(2) >= c.batch.max_seq_len && t->size(2) <= INT32_MAX;
+}
+inline at::Tensor bytes_like(const at::Tensor& t, size_t n) { return at::empty({(int64_t)(n ? n : 16)}, t.options().dtype(at::kByte)); }
+
+// Tickets of the current stream: made once a stream and kept in `by_stream`; a captured call has some of its own, cleared at
+// every replay, since two graphs may run at the same time.
+at::Tensor tickets_of(PyObject* by_stream, const at::Tensor& like) {
+    auto make = [&] { return at::zeros({(int64_t)tq_pages_ticket_bytes()}, like.options().dtype(at::kByte)); };
+    if (capturing(like)) return make();
+    PyObject* key = PyLong_FromVoidPtr(stream_of(like));
+    if (key == nullptr) throw python_error();
+    PyObject* have = PyDict_GetItemWithError(by_stream, key);      // borrowed
+    const at::Tensor* t = have ? tensor_or_null(have) : nullptr;
+    at::Tensor res;
+    if (t) {
+        res = *t;
+    } else if (!PyErr_Occurred()) {
+        res = make();
+        PyObject* value = THPVariable_Wrap(res);
+        if (value == nullptr || PyDict_SetItem(by_stream, key, value) != 0) PyErr_Clear();
+        Py_XDECREF(value);
+    }
+    Py_DECREF(key);
+    if (PyErr_Occurred()) throw python_error();
+    return res;
+}
+
+// pages_write(pages, status, key, value, slots) -> status code or None
+PyObject* pages_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    ARGS(5);
+    const tq_pages* g = address<const tq_pages>(args[0]);
+    const at::Tensor *status = tensor_or_null(args[1]), *k = tensor_or_null(args[2]), *v = tensor_or_null(args[3]), *slots = tensor_or_null(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!status || !k || !v || !slots || !rows_ok(*k, g->num_kv_heads, g->head_dim) || !rows_ok(*v, g->num_kv_heads, g->head_dim) ||
+        !on(*k, *status) || !on(*v, *status) || !on(*slots, *status) || dtype_code(k->scalar_type()) != (int)g->dtype ||
+        v->scalar_type() != k->scalar_type() || k->size(0) != v->size(0) || slots->dim() != 1 || slots->scalar_type() != at::kLong ||
+        slots->size(0) < k->size(0) || !slots->is_contiguous() || k->size(0) < 1)
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(status->get_device());
+    const int rc = tq_pages_write(g, k->data_ptr(), v->data_ptr(), k->size(0), k->stride(0), k->stride(1), v->stride(0), v->stride(1),
+                                  slots->data_ptr<int64_t>(), status->data_ptr<int32_t>(), stream_of(*status));
+    if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
+    return PyLong_FromLong(rc);
+    END_HANDLE_TH_ERRORS
+}
+
+// pages_decode(pages, status, tickets by stream, query (b, Qh, D), tables, lens, max_len, scale | None, out | None, mass | None)
+//   -> out, status code, or None
+PyObject* pages_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    ARGS(10);
+    const at::Tensor *q = tensor_or_null(args[3]), *out = tensor_or_null(args[8]), *mass = tensor_or_null(args[9]);
+    PagesCall c;
+    if (!q || q->dim() != 3 || !pages_call(c, args[0], args[1], args[4], args[5], args[6], q->size(0))) {
+        if (PyErr_Occurred()) return nullptr;
+        Py_RETURN_NONE;
+    }
+    const int64_t d = c.pages->head_dim, qh = q->size(1);
+    const double scale = args[7] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!on(*q, *c.status) || !q->is_contiguous() || q->size(2) != d || qh < 1 || qh > INT32_MAX || dtype_code(q->scalar_type()) != (int)c.pages->dtype ||
+        (out && (!on(*out, *c.status) || !out->is_contiguous() || out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type())) ||
+        (args[9] != Py_None && !plane_ok(mass, c, at::kFloat)) || !PyDict_Check(args[2]))
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(c.status->get_device());
+    size_t need = 0;
+    int rc = tq_pages_decode_scratch_bytes(c.pages, &c.batch, (int32_t)qh, mass ? 1 : 0, &need);
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    const at::Tensor scratch = bytes_like(*q, need), tickets = tickets_of(args[2], *c.status);
+    at::Tensor res;
+    if (!out) {
+        res = at::empty_like(*q);
+        out = &res;
+    }
+    rc = tq_pages_decode(c.pages, &c.batch, q->data_ptr(), (int32_t)qh, (float)scale, out->data_ptr(), mass ? mass->data_ptr<float>() : nullptr,
+                         mass ? mass->size(2) : 0, scratch.data_ptr(), need, reinterpret_cast<int32_t*>(tickets.data_ptr()),
+                         c.status->data_ptr<int32_t>(), stream_of(*q));
+    if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    if (!res.defined()) {
+        Py_INCREF(args[8]);
+        return args[8];
+    }
+    return THPVariable_Wrap(std::move(res));
+    END_HANDLE_TH_ERRORS
+}
+
+// pages_observe(pages, status, query (b, window, Qh, D), tables, lens, max_len, scale | None, mass) -> status code or None
+PyObject* pages_observe(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    ARGS(8);
+    const at::Tensor *q = tensor_or_null(args[2]), *mass = tensor_or_null(args[7]);
+    PagesCall c;
+    if (!q || q->dim() != 4 || !pages_call(c, args[0], args[1], args[3], args[4], args[5], q->size(0))) {
+        if (PyErr_Occurred()) return nullptr;
+        Py_RETURN_NONE;
+    }
+    const int64_t d = c.pages->head_dim, qh = q->size(2), window = q->size(1);
+    const double scale = args[6] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!on(*q, *c.status) || !q->is_contiguous() || q->size(3) != d || qh < 1 || qh > INT32_MAX || window < 1 || window > INT32_MAX ||
+        dtype_code(q->scalar_type()) != (int)c.pages->dtype || !plane_ok(mass, c, at::kFloat))
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(c.status->get_device());
+    size_t need = 0;
+    int rc = tq_pages_observe_scratch_bytes(c.pages, &c.batch, (int32_t)window, (int32_t)qh, &need);
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    const at::Tensor scratch = bytes_like(*q, need);
+    rc = tq_pages_observe(c.pages, &c.batch, q->data_ptr(), (int32_t)window, (int32_t)qh, (float)scale, mass->data_ptr<float>(), mass->size(2),
+                          scratch.data_ptr(), need, c.status->data_ptr<int32_t>(), stream_of(*q));
+    if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
+    return PyLong_FromLong(rc);
+    END_HANDLE_TH_ERRORS
+}
+
+// mass, positions, held, seen
+bool ledger_of(tq_pages_ledger& l, const PagesCall& c, PyObject* const* args) {
+    const at::Tensor *mass = tensor_or_null(args[0]), *pos = tensor_or_null(args[1]), *held = tensor_or_null(args[2]), *seen = tensor_or_null(args[3]);
+    if (!plane_ok(mass, c, at::kFloat) || !plane_ok(pos, c, at::kInt) || pos->size(2) != mass->size(2)) return false;
+    for (const at::Tensor* t : {held, seen})
+        if (!t || !on(*t, *c.status) || t->dim() != 1 || t->scalar_type() != at::kInt || t->size(0) < c.batch.batch || !t->is_contiguous()) return false;
+    l.mass = mass->data_ptr<float>();
+    l.positions = pos->data_ptr<int32_t>();
+    l.held = held->data_ptr<int32_t>();
+    l.seen = seen->data_ptr<int32_t>();
+    l.max_tokens = (int32_t)mass->size(2);
+    return true;
+}
+
+// pages_evict(pages, status, tables, lens, max_len, budget, recent, 4 tensors of the ledger, 4 of the one to write) -> new lengths,
+// status code, or None
+PyObject* pages_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    ARGS(15);
+    const at::Tensor* lens = tensor_or_null(args[3]);
+    const int64_t budget = PyLong_AsLongLong(args[5]), recent = PyLong_AsLongLong(args[6]);
+    PagesCall c;
+    tq_pages_ledger from = {}, to = {};
+    if (PyErr_Occurred()) return nullptr;
+    if (!lens || lens->dim() != 1 || !pages_call(c, args[0], args[1], args[2], args[3], args[4], lens->size(0)) || budget < 0 || budget > INT32_MAX ||
+        recent < 0 || recent > INT32_MAX || !ledger_of(from, c, args + 7) || !ledger_of(to, c, args + 11)) {
+        if (PyErr_Occurred()) return nullptr;
+        Py_RETURN_NONE;
+    }
+    const c10::cuda::CUDAGuard guard(c.status->get_device());
+    size_t need = 0;
+    int rc = tq_pages_evict_scratch_bytes(c.pages, &c.batch, (int32_t)budget, &need);
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    const at::Tensor scratch = bytes_like(*lens, need);
+    at::Tensor after = at::empty_like(*lens);
+    rc = tq_pages_evict(c.pages, &c.batch, &from, &to, (int32_t)budget, (int32_t)recent, after.data_ptr<int32_t>(), scratch.data_ptr(), need,
+                        c.status->data_ptr<int32_t>(), stream_of(*lens));
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(std::move(after));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"pages_write", (PyCFunction)(void (*)(void))pages_write, METH_FASTCALL, nullptr},
+    {"pages_decode", (PyCFunction)(void (*)(void))pages_decode, METH_FASTCALL, nullptr},
+    {"pages_observe", (PyCFunction)(void (*)(void))pages_observe, METH_FASTCALL, nullptr},
+    {"pages_evict", (PyCFunction)(void (*)(void))pages_evict, METH_FASTCALL, nullptr},
     {"cache_scores", (PyCFunction)(void (*)(void))cache_scores, METH_FASTCALL, nullptr},
     {"cache_attend", (PyCFunction)(void (*)(void))cache_attend, METH_FASTCALL, nullptr},
     {"quantize_keys", (PyCFunction)(void (*)(void))quantize_keys, METH_FASTCALL, nullptr},

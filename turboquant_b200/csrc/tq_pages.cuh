@@ -1,0 +1,68 @@
+// The exact paged cache: what its kernels share.  A page holds `page` tokens of every kv head as 16-bit key and value rows;
+// element (block, token, head, :) of a plane is at block * sb + token * st + head * sh (bytes here), rows 16-byte aligned.
+#pragma once
+#include "tq_common.cuh"
+
+namespace tqpg {
+
+struct Pages {
+    uint8_t* k;
+    uint8_t* v;
+    int64_t num_blocks;
+    int64_t sb, st, sh;   // bytes
+    int page, H;
+};
+struct Batch {
+    const int32_t* table;
+    const int32_t* lens;
+    int table_stride, batch, max_seq_len;
+};
+
+// Longest table index a length may reach is checked on the host (max_seq_len against the table's width); a length outside
+// [0, max_seq_len] is clamped and reported.
+__device__ __forceinline__ int seq_len(const Batch& q, int b, int32_t* status) {
+    const int n = q.lens[b];
+    if (n >= 0 && n <= q.max_seq_len) return n;
+    atomicCAS(status, 0, (int)TQ_ERR_RANGE);
+    return n < 0 ? 0 : q.max_seq_len;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes to shared memory, zeros where `ok` is false (nothing is read then)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+inline int pages_check(const tq_pages* g) {
+    if (!g || !g->key || !g->value) return TQ_ERR_NULL;
+    if (g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256) return TQ_ERR_UNSUPPORTED;
+    if (g->dtype != TQ_BF16 && g->dtype != TQ_F16) return TQ_ERR_UNSUPPORTED;
+    if (g->num_blocks < 1 || g->block_size < 1 || g->num_kv_heads < 1 || g->num_kv_heads > 65535) return TQ_ERR_SHAPE;
+    if (g->num_blocks >= ((int64_t)1 << 31)) return TQ_ERR_SHAPE;
+    if (((uintptr_t)g->key & 15) || ((uintptr_t)g->value & 15) || (g->stride_block & 7) || (g->stride_token & 7) || (g->stride_head & 7))
+        return TQ_ERR_ALIGN;
+    if (g->stride_block < 0 || g->stride_token < 0 || g->stride_head < 0) return TQ_ERR_SHAPE;
+    return TQ_OK;
+}
+inline Pages pages_of(const tq_pages* g) {
+    return Pages{static_cast<uint8_t*>(g->key), static_cast<uint8_t*>(g->value), g->num_blocks, g->stride_block * 2,
+                 g->stride_token * 2, g->stride_head * 2, g->block_size, g->num_kv_heads};
+}
+// A batch has at most 2^31 units of 16 tokens and head, and a table row covers max_seq_len tokens.
+inline int batch_check(const tq_pages* g, const tq_pages_batch* q) {
+    if (!q || !q->block_tables || !q->seq_lens) return TQ_ERR_NULL;
+    if (q->batch < 1 || q->max_seq_len < 1 || q->table_width < 1 || q->table_stride < q->table_width) return TQ_ERR_SHAPE;
+    if ((int64_t)q->table_width * g->block_size < q->max_seq_len || q->max_seq_len > (1 << 30)) return TQ_ERR_RANGE;
+    return TQ_OK;
+}
+inline Batch batch_of(const tq_pages_batch* q) {
+    return Batch{q->block_tables, q->seq_lens, q->table_stride, q->batch, q->max_seq_len};
+}
+
+}  // namespace tqpg
