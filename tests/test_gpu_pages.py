@@ -360,6 +360,26 @@ def test_evict_reports_a_bad_page_and_moves_the_rest():
     assert torch.equal(rows(s.cache.key_cache)[:16], rows(before)[32:48]) and torch.equal(rows(s.cache.key_cache)[16:], rows(before)[16:])
 
 
+def test_every_token_is_counted_once():
+    """Lengths that put the borders of shares, warps and sequences in all places to each other: a step's weights sum to the
+    number of query heads, and the outputs follow for values that are all ones."""
+    rng = random.Random(17)
+    for i in range(60):
+        D, H, G = rng.choice((64, 128, 256)), rng.randint(1, 3), rng.choice((1, 4, 8, 11))
+        top = rng.choice((60, 400, 3000, 20000))
+        lens = [rng.randint(1, top) for _ in range(rng.choice((1, 2, 3, 9, 33)))]
+        while sum(lens) > 60000:
+            lens.pop()
+        s = Setup(lens, H, D, rng.choice((16, 64)), seed=i)
+        ones = torch.ones_like(s.cache.value_cache)
+        cache = PagedKVCache(s.spec, s.cache.key_cache, ones)
+        led = AttentionLedger(len(lens), H, s.longest, "cuda")
+        out = cache.decode(s.query(len(lens), heads=H * G).cuda(), s.dtable, s.dlens, s.longest, ledger=led)
+        # weights are off by 2^-20 or so each, sums of up to 20000 of them in 64 bits
+        assert ((led.mass.double().sum(-1) - G).abs() <= G * 2.0 ** -15).all(), (i, lens)
+        assert ((out.double() - 1).abs() <= 2.0 ** -8).all() and cache.status() == 0
+
+
 def test_two_captured_graphs_and_an_eager_stream_at_once():
     """Calls captured twice and replayed at the same time, beside eager calls on a third stream: each has memory of its own."""
     s = Setup([9000, 4000], 2, 128, seed=12)

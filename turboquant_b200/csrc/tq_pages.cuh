@@ -5,12 +5,26 @@
 
 namespace tqpg {
 
+// Quotients of numbers below 2^31 by a number that the host knows: q = n * mul >> (31 + shift), exact for mul = ceil(2^(31 + shift) / d)
+// with 2^shift >= d, since the excess of mul is below 2^shift / 2^(31 + shift) a unit of n.
+struct Divisor {
+    uint32_t mul;
+    int shift, d;
+    __device__ __forceinline__ int quotient(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> (31 + shift)); }
+};
+inline Divisor divisor(int d) {
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    return Divisor{(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), s, d};
+}
+
 struct Pages {
     uint8_t* k;
     uint8_t* v;
     int64_t num_blocks;
     int64_t sb, st, sh;   // bytes
     int page, H;
+    Divisor by_page;
 };
 struct Batch {
     const int32_t* table;
@@ -39,6 +53,23 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Launch as a programmatic dependent: the CTAs may take their places while the launch ahead finishes.  Every kernel launched so
+// waits for it before it reads or writes anything, and lets the launch behind begin only after that.
+template <class... P, class... A>
+inline int launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? TQ_OK : TQ_ERR_CUDA;
+}
+
 inline int pages_check(const tq_pages* g) {
     if (!g || !g->key || !g->value) return TQ_ERR_NULL;
     if (g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256) return TQ_ERR_UNSUPPORTED;
@@ -52,7 +83,7 @@ inline int pages_check(const tq_pages* g) {
 }
 inline Pages pages_of(const tq_pages* g) {
     return Pages{static_cast<uint8_t*>(g->key), static_cast<uint8_t*>(g->value), g->num_blocks, g->stride_block * 2,
-                 g->stride_token * 2, g->stride_head * 2, g->block_size, g->num_kv_heads};
+                 g->stride_token * 2, g->stride_head * 2, g->block_size, g->num_kv_heads, divisor(g->block_size)};
 }
 // A batch has at most 2^31 units of 16 tokens and head, and a table row covers max_seq_len tokens.
 inline int batch_check(const tq_pages* g, const tq_pages_batch* q) {
