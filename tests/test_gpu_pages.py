@@ -251,6 +251,30 @@ def test_observe(lens, W, H, G, D, page, dtype):
         assert ((mass[b, :, :n] - before[b, :, :n] - add).abs() <= add * (rel + many) + (mass[b, :, :n]) * 2.0 ** -23 * (1 + W * G // 128)).all()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.3])
+def test_scales_of_either_sign(scale):
+    """No scale at all (equal weights), a negative one, a large one; the last tile is a partial one and has a bad page."""
+    s = Setup([300, 129], 2, 128, seed=14)
+    table = s.table.clone()
+    table[0, 3] = -1
+    there = torch.ones(300, dtype=torch.bool)
+    there[48:64] = False
+    q = s.query(2, 4, heads=8)
+    a, b = AttentionLedger(2, 2, s.longest, "cuda"), AttentionLedger(2, 2, s.longest, "cuda")
+    s.cache.observe(q.cuda(), table.cuda(), s.dlens, s.longest, a, scale=scale)
+    out = s.cache.decode(q[:, 3].cuda(), table.cuda(), s.dlens, s.longest, scale=scale, ledger=b).cpu().double()
+    for i, n in enumerate(s.lens):
+        k, v = s.rows(i)
+        ok = there[:n] if i == 0 else torch.ones(n, dtype=torch.bool)
+        rel = weight_error(q.double(), k, abs(scale))
+        _, p = O.attention(q[i].double().view(4, 2, 4, 128), k, v, scale=scale, last=torch.arange(n - 4, n), there=ok)
+        ref, p1 = O.attention(q[i, 3].double().view(1, 2, 4, 128), k, v, scale=scale, there=ok)
+        check_out(out[i].view(1, 2, 4, 128), ref, p1, v, BF16, rel)
+        for led, add in ((a, p.sum((0, 2))), (b, p1[0].sum(1))):
+            assert ((led.mass[i, :, :n].cpu().double() - add).abs() <= add * (rel + 2.0 ** -19)).all()
+    assert s.cache.status() == RANGE
+
+
 def test_observing_one_query_is_what_decode_adds():
     s = Setup([400, 77], 2, 128, seed=4)
     q = s.query(2, heads=8).cuda()
