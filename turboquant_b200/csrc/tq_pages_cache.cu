@@ -23,6 +23,8 @@ struct WriteParams {
 template <int D>
 __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteParams p) {
     constexpr int CH = D / 8;                              // 16-byte pieces of a row
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int pieces = p.g.H * CH;
     const int64_t t0 = (int64_t)blockIdx.x * WR_TOK;
     for (int i = threadIdx.x; i < 2 * pieces; i += WR_THREADS) {
@@ -55,9 +57,10 @@ __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteP
 
 // One CTA settles a (sequence, kv head): which slots are kept, the ledger, and the list of moves; a second launch moves the
 // rows.  Order of keeping: protected tokens, then mass as a 32-bit key with the order of the numbers.  The k-th largest key is
-// found bit by bit from the top, by counting the keys that reach a trial value - no histogram, so nothing depends on how the
-// weights spread (they differ by a few powers of two, and the counters of a histogram would be hit by all lanes at once).
-// Lane-striped slots (warp * 32 * KPT + i * 32 + lane) let a ballot count a row and keep every list in ascending order.
+// found bit by bit, from the highest one in which the candidates differ, by counting the keys that reach a trial value - no
+// histogram, so nothing depends on how the weights spread (they differ by a few powers of two, and the counters of a histogram
+// would be hit by all lanes at once).  A trial costs two instructions a key and one exchange between the warps.  Lane-striped
+// slots (warp * 32 * KPT + i * 32 + lane) let a ballot count a row and keep every list in ascending order.
 struct EvictParams {
     Pages g;
     Batch q;
@@ -83,39 +86,36 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the CTA of a value that is the same in all lanes of a warp; two buffers in turn, one barrier.
-template <int NW>
+// Exchange of one number a warp; two buffers in turn, one barrier.
 struct CtaSum {
-    int* buf;      // [2][NW]
-    int turn;
-    __device__ __forceinline__ int operator()(int x) {
-        int* b = buf + (turn & 1) * NW;
+    int* buf;      // [2][32]
+    int turn, warps;
+    __device__ __forceinline__ int all_of(int x) {         // what the lane's warp gave
+        int* b = buf + (turn & 1) * 32;
         turn ^= 1;
-        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = x;
-        __syncthreads();
         const int lane = threadIdx.x & 31;
-        return __reduce_add_sync(0xffffffffu, lane < NW ? b[lane] : 0);
-    }
-    // ... of the warps before this one, and of all
-    __device__ __forceinline__ int before(int x, int& total) {
-        int* b = buf + (turn & 1) * NW;
-        turn ^= 1;
-        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-        if (lane == 0) b[w] = x;
+        if (lane == 0) b[threadIdx.x >> 5] = x;
         __syncthreads();
-        const int y = lane < NW ? b[lane] : 0;
+        return lane < warps ? b[lane] : 0;
+    }
+    __device__ __forceinline__ int operator()(int x) { return __reduce_add_sync(0xffffffffu, all_of(x)); }
+    // the sum of the warps before this one, and of all
+    __device__ __forceinline__ int before(int x, int& total) {
+        const int y = all_of(x), lane = threadIdx.x & 31;
         total = __reduce_add_sync(0xffffffffu, y);
-        return __reduce_add_sync(0xffffffffu, lane < w ? y : 0);
+        return __reduce_add_sync(0xffffffffu, lane < (int)(threadIdx.x >> 5) ? y : 0);
     }
 };
 
-// NW warps, KPT slots a thread: up to NW * 32 * KPT tokens at a time in registers; longer rows are gone over again for every
-// count (LONG).
-template <int NW, int KPT, bool LONG>
-__global__ void __launch_bounds__(NW * 32) tq_pages_evict_kernel(const EvictParams p) {
-    __shared__ int s_buf[2 * NW];
-    const int row = blockIdx.x, b = row / p.g.H, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// KPT slots a thread, held as keys in registers; a row that is longer than all threads hold (LONG) is gone over again for every
+// count.  Masses and positions are read again where they are written: they are in the caches.
+template <int KPT, bool LONG>
+__global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams p) {
+    __shared__ int s_buf[64];
+    const int row = blockIdx.x, b = row / p.g.H, lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t below = (1u << lane) - 1u;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = seq_len(p.q, b, p.status), m = min(n, p.budget);
     const int held = p.held[b], seen = p.seen[b], late = seen + n - held - p.recent;
     const float* mass = p.mass + row * p.stride;
@@ -123,50 +123,81 @@ __global__ void __launch_bounds__(NW * 32) tq_pages_evict_kernel(const EvictPara
     float* out_mass = p.out_mass + row * p.out_stride;
     int32_t* out_positions = p.out_positions + row * p.out_stride;
     int32_t *dst = p.dst + (int64_t)row * p.list, *src = p.src + (int64_t)row * p.list;
-    CtaSum<NW> sum{s_buf, 0};
-    constexpr int SPAN = NW * 32 * KPT;
-    const int rounds = LONG ? (n + SPAN - 1) / SPAN : 1;
+    CtaSum sum{s_buf, 0, warps};
+    const int span = warps * 32 * KPT, rounds = LONG ? (n + span - 1) / span : 1;
 
-    float x[KPT];
-    int pos[KPT];
     uint32_t key[KPT];                 // 0: not in the cache
-    auto slot_of = [&](int r, int i) { return r * SPAN + (w * KPT + i) * 32 + lane; };
+    uint32_t guard = 0;                // bit i: slot i of this thread is protected
+    auto slot_of = [&](int r, int i) { return r * span + (w * KPT + i) * 32 + lane; };
+    auto position = [&](int t) { return t < held ? positions[t] : seen + t - held; };
     auto load = [&](int r) {
+        const int t0 = slot_of(r, 0);
+        guard = 0;
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const int t = slot_of(r, i);
-            x[i] = t < n ? mass[t] : 0.f;
-            pos[i] = t < n && t < held ? positions[t] : seen + t - held;
+        for (int c = 0; c < KPT; c += 8) {                 // eight at a time: more would not fit the registers
+            float x[8];
+            int pos[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = t0 + (c + i) * 32 < n ? mass[t0 + (c + i) * 32] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pos[i] = t0 + (c + i) * 32 < n ? position(t0 + (c + i) * 32) : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool there = t0 + (c + i) * 32 < n;
+                key[c + i] = there ? key_of(x[i]) : 0u;
+                guard |= (uint32_t)(there && pos[i] >= late) << (c + i);
+            }
+            asm volatile("" ::: "memory");
         }
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) key[i] = slot_of(r, i) < n ? key_of(x[i]) : 0u;
     };
     load(0);
 
     // protected tokens first; the rest by key, or the protected by key where they alone exceed the budget
-    int guarded = 0;
-    if (n > m) {
+    const bool trims = n > m;
+    bool all_guarded = false;          // the candidates are the protected tokens
+    uint32_t limit = 0u;               // the k-th largest key of the candidates
+    int equal_taken = 0;               // how many of the keys equal to it are taken, lowest slots first
+    auto among = [&](int i) { return ((guard >> i) & 1u) == (uint32_t)all_guarded; };
+    if (trims) {
+        int guarded = 0;
         for (int r = 0; r < rounds; ++r) {
             if (LONG && r > 0) load(r);
-#pragma unroll
-            for (int i = 0; i < KPT; ++i) guarded += key[i] != 0u && pos[i] >= late;
+            guarded += __popc(guard);
         }
         guarded = sum(__reduce_add_sync(0xffffffffu, guarded));
-    }
-    const bool all_guarded = guarded >= m;                 // candidates: the protected ones / the others
-    const int k = all_guarded ? m : m - guarded;
-    auto candidate = [&](int i) { return key[i] != 0u && (pos[i] >= late) == all_guarded; };
-    uint32_t limit = 0u;                                   // the k-th largest key of the candidates
-    int equal_taken = 0;                                   // how many of the keys equal to it are taken, lowest slots first
-    if (n > m) {
-        int reach = -1;                                    // keys >= limit
-        for (int bit = 31; bit >= 0 && reach != k; --bit) {
+        all_guarded = guarded >= m;
+        const int k = all_guarded ? m : m - guarded;
+        // keys of others than candidates are 0 from here on, and no trial value is
+        uint32_t ones = 0xffffffffu, any = 0u;
+        auto drop = [&]() {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)
+                if (!among(i)) key[i] = 0u;
+        };
+        for (int r = 0; r < rounds; ++r) {
+            if (LONG) load(r);
+            drop();
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)
+                if (key[i] != 0u) ones &= key[i], any |= key[i];
+        }
+        ones = (uint32_t)sum.all_of((int)__reduce_and_sync(0xffffffffu, ones));
+        any = (uint32_t)sum.all_of((int)__reduce_or_sync(0xffffffffu, any));
+        ones = __reduce_and_sync(0xffffffffu, lane < warps ? ones : 0xffffffffu);
+        any = __reduce_or_sync(0xffffffffu, any);
+        const uint32_t differ = ones ^ any;
+        int bit = 31 - __clz(differ), reach = -1;          // reach: keys >= limit
+        limit = differ == 0u ? any : bit == 31 ? 0u : any >> (bit + 1) << (bit + 1);       // what all candidates have in common
+        for (; bit >= 0 && reach != k; --bit) {
             const uint32_t trial = limit | (1u << bit);
             int c = 0;
             for (int r = 0; r < rounds; ++r) {
-                if (LONG) load(r);
+                if (LONG) {
+                    load(r);
+                    drop();
+                }
 #pragma unroll
-                for (int i = 0; i < KPT; ++i) c += candidate(i) && key[i] >= trial;
+                for (int i = 0; i < KPT; ++i) c += key[i] >= trial;
             }
             c = sum(__reduce_add_sync(0xffffffffu, c));
             if (c >= k) {
@@ -174,49 +205,57 @@ __global__ void __launch_bounds__(NW * 32) tq_pages_evict_kernel(const EvictPara
                 reach = c;
             }
         }
-        int above = 0;
-        for (int r = 0; r < rounds; ++r) {
-            if (LONG) load(r);
+        if (k == 0) {                                      // nothing but the protected ones
+            limit = 0xffffffffu;
+        } else if (reach == k) {
+            equal_taken = 0x7fffffff;
+        } else {
+            int above = 0;
+            for (int r = 0; r < rounds; ++r) {
+                if (LONG) {
+                    load(r);
+                    drop();
+                }
 #pragma unroll
-            for (int i = 0; i < KPT; ++i) above += candidate(i) && key[i] > limit;
+                for (int i = 0; i < KPT; ++i) above += key[i] > limit;
+            }
+            equal_taken = k - sum(__reduce_add_sync(0xffffffffu, above));
         }
-        above = sum(__reduce_add_sync(0xffffffffu, above));
-        equal_taken = reach == k ? 0x7fffffff : k - above;
-        if (k == 0) equal_taken = 0, limit = 0xffffffffu;  // nothing but the protected ones
     }
 
     // the lists, in ascending order: holes before m, movers behind it
     int equals = 0, holes = 0, movers = 0;                 // of the slots before this round
     for (int r = 0; r < rounds; ++r) {
-        if (LONG) load(r);
-        uint32_t eq[KPT];
-        int mine = 0, total;
+        if (LONG) {
+            load(r);
+            if (trims) {
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            eq[i] = __ballot_sync(0xffffffffu, n > m && candidate(i) && key[i] == limit);
-            mine += __popc(eq[i]);
+                for (int i = 0; i < KPT; ++i)
+                    if (!among(i)) key[i] = 0u;
+            }
+        }
+        const int t0 = slot_of(r, 0);
+        int mine = 0, total;
+        if (trims) {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) mine += __popc(__ballot_sync(0xffffffffu, key[i] != 0u && key[i] == limit));
         }
         int rank = equals + sum.before(mine, total);
         equals += total;
-        uint32_t hole[KPT], mover[KPT];
+        uint32_t kept = 0;                                 // bit i: slot i of this thread stays in the cache
         int my_holes = 0, my_movers = 0;
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            const int t = slot_of(r, i);
-            bool kept = key[i] != 0u;
-            if (n > m) {
-                const bool c = candidate(i);
-                kept = kept && (c ? key[i] > limit || (key[i] == limit && rank + __popc(eq[i] & below) < equal_taken) : !all_guarded);
+            const int t = t0 + i * 32;
+            bool stays = t < n;
+            if (trims) {
+                const uint32_t eq = __ballot_sync(0xffffffffu, key[i] != 0u && key[i] == limit);
+                stays = stays && (among(i) ? key[i] > limit || (key[i] == limit && rank + __popc(eq & below) < equal_taken) : !all_guarded);
+                rank += __popc(eq);
             }
-            rank += __popc(eq[i]);
-            hole[i] = __ballot_sync(0xffffffffu, t < m && !kept);
-            mover[i] = __ballot_sync(0xffffffffu, t >= m && kept);
-            my_holes += __popc(hole[i]);
-            my_movers += __popc(mover[i]);
-            if (t < m && kept) {
-                out_mass[t] = x[i];
-                out_positions[t] = pos[i];
-            }
+            my_holes += __popc(__ballot_sync(0xffffffffu, t < m && !stays));
+            my_movers += __popc(__ballot_sync(0xffffffffu, t >= m && stays));
+            kept |= (uint32_t)stays << i;
         }
         int total_holes, total_movers;
         int hole_at = holes + sum.before(my_holes, total_holes), mover_at = movers + sum.before(my_movers, total_movers);
@@ -224,24 +263,33 @@ __global__ void __launch_bounds__(NW * 32) tq_pages_evict_kernel(const EvictPara
         movers += total_movers;
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            if ((hole[i] >> lane) & 1) dst[hole_at + __popc(hole[i] & below)] = slot_of(r, i);
-            hole_at += __popc(hole[i]);
+            const int t = t0 + i * 32;
+            const bool stays = (kept >> i) & 1;
+            const uint32_t hole = __ballot_sync(0xffffffffu, t < m && !stays);
+            if (t < m && !stays) dst[hole_at + __popc(hole & below)] = t;
+            hole_at += __popc(hole);
+            if (t < m && stays) {
+                out_mass[t] = mass[t];
+                out_positions[t] = position(t);
+            }
         }
         __syncthreads();                                   // every hole that a mover of this round takes has been noted: holes lie before movers
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            if ((mover[i] >> lane) & 1) {
-                const int j = mover_at + __popc(mover[i] & below);
-                const int to = dst[j];
-                src[j] = slot_of(r, i);
-                out_mass[to] = x[i];
-                out_positions[to] = pos[i];
+            const int t = t0 + i * 32;
+            const bool moves = t >= m && ((kept >> i) & 1);
+            const uint32_t mover = __ballot_sync(0xffffffffu, moves);
+            if (moves) {
+                const int j = mover_at + __popc(mover & below), to = dst[j];
+                src[j] = t;
+                out_mass[to] = mass[t];
+                out_positions[to] = position(t);
             }
-            mover_at += __popc(mover[i]);
+            mover_at += __popc(mover);
         }
     }
     __syncthreads();                                       // in place: nothing is cleared before it has been read
-    for (int64_t t = m + (int)threadIdx.x; t < p.out_stride; t += NW * 32) {
+    for (int64_t t = m + (int)threadIdx.x; t < p.out_stride; t += blockDim.x) {
         out_mass[t] = 0.f;
         out_positions[t] = -1;
     }
@@ -252,6 +300,7 @@ __global__ void __launch_bounds__(NW * 32) tq_pages_evict_kernel(const EvictPara
 template <int D>
 __global__ void __launch_bounds__(256) tq_pages_move_kernel(const EvictParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int LPR = D / 8, PER = 256 / LPR;
     const int row = blockIdx.x, b = row / p.g.H, h = row % p.g.H;
     if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) {   // here, not in the first launch: other heads of the sequence read them there
@@ -308,11 +357,10 @@ extern "C" int tq_pages_write(const tq_pages* pages, const void* key, const void
     cudaStream_t st = (cudaStream_t)stream;
     tq_note_launch(st, TQ_LAUNCH_WAITED);      // writes rows that a store may read next
     switch (pages->head_dim) {
-        case 64: tq_pages_write_kernel<64><<<(unsigned)ctas, WR_THREADS, 0, st>>>(p); break;
-        case 128: tq_pages_write_kernel<128><<<(unsigned)ctas, WR_THREADS, 0, st>>>(p); break;
-        default: tq_pages_write_kernel<256><<<(unsigned)ctas, WR_THREADS, 0, st>>>(p); break;
+        case 64: return launch_behind(tq_pages_write_kernel<64>, dim3((unsigned)ctas), WR_THREADS, 0, st, p);
+        case 128: return launch_behind(tq_pages_write_kernel<128>, dim3((unsigned)ctas), WR_THREADS, 0, st, p);
+        default: return launch_behind(tq_pages_write_kernel<256>, dim3((unsigned)ctas), WR_THREADS, 0, st, p);
     }
-    return cudaGetLastError() == cudaSuccess ? TQ_OK : TQ_ERR_CUDA;
 }
 
 extern "C" int tq_pages_evict_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t budget, size_t* out) {
@@ -363,17 +411,19 @@ extern "C" int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch
     cudaStream_t st = (cudaStream_t)stream;
     tq_note_launch(st, TQ_LAUNCH_WAITED);      // writes rows that a store may read next
     const int n = batch->max_seq_len;
-    if (n <= 8 * 32 * 8) tq_pages_evict_kernel<8, 8, false><<<(unsigned)rows, 256, 0, st>>>(p);
-    else if (n <= 32 * 32 * 8) tq_pages_evict_kernel<32, 8, false><<<(unsigned)rows, 1024, 0, st>>>(p);
-    else tq_pages_evict_kernel<32, 8, true><<<(unsigned)rows, 1024, 0, st>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return TQ_ERR_CUDA;
+    auto threads_for = [&](int kpt) { return n >= 1024 * kpt ? 1024 : (n + 32 * kpt - 1) / (32 * kpt) * 32; };
+    int rc2;
+    // eight keys a thread as far as 1024 threads hold the row, then thirty-two
+    if (n <= 1024 * 8) rc2 = launch_behind(tq_pages_evict_kernel<8, false>, dim3((unsigned)rows), threads_for(8), 0, st, p);
+    else if (n <= 1024 * 32) rc2 = launch_behind(tq_pages_evict_kernel<32, false>, dim3((unsigned)rows), threads_for(32), 0, st, p);
+    else rc2 = launch_behind(tq_pages_evict_kernel<32, true>, dim3((unsigned)rows), 1024, 0, st, p);
+    if (rc2 != TQ_OK) return rc2;
     const int per = 256 / (pages->head_dim / 8);
     const int64_t tiles = (p.list + per - 1) / per;
     const dim3 grid((unsigned)rows, (unsigned)(tiles < 1 ? 1 : tiles > 1024 ? 1024 : tiles));
     switch (pages->head_dim) {
-        case 64: tq_pages_move_kernel<64><<<grid, 256, 0, st>>>(p); break;
-        case 128: tq_pages_move_kernel<128><<<grid, 256, 0, st>>>(p); break;
-        default: tq_pages_move_kernel<256><<<grid, 256, 0, st>>>(p); break;
+        case 64: return launch_behind(tq_pages_move_kernel<64>, grid, 256, 0, st, p);
+        case 128: return launch_behind(tq_pages_move_kernel<128>, grid, 256, 0, st, p);
+        default: return launch_behind(tq_pages_move_kernel<256>, grid, 256, 0, st, p);
     }
-    return cudaGetLastError() == cudaSuccess ? TQ_OK : TQ_ERR_CUDA;
 }
