@@ -56,18 +56,29 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // Launch as a programmatic dependent: the CTAs may take their places while the launch ahead finishes.  Every kernel launched so
 // waits for it before it reads or writes anything, and lets the launch behind begin only after that.
 template <class... P, class... A>
-inline int launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+inline int launch_behind_as(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? TQ_OK : TQ_ERR_CUDA;
+}
+template <class... P, class... A>
+inline int launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    return launch_behind_as(kernel, grid, threads, smem, 1, st, args...);
+}
+template <class... P, class... A>
+inline int launch_behind_in_clusters(void (*kernel)(P...), dim3 grid, int threads, int cluster, cudaStream_t st, A... args) {
+    return launch_behind_as(kernel, grid, threads, 0, cluster, st, args...);
 }
 
 inline int pages_check(const tq_pages* g) {

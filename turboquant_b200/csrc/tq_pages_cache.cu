@@ -55,12 +55,13 @@ __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteP
 
 // ---------------------------------------------------------------------------------------------------------------- evict
 
-// One CTA settles a (sequence, kv head): which slots are kept, the ledger, and the list of moves; a second launch moves the
-// rows.  Order of keeping: protected tokens, then mass as a 32-bit key with the order of the numbers.  The k-th largest key is
-// found bit by bit, from the highest one in which the candidates differ, by counting the keys that reach a trial value - no
-// histogram, so nothing depends on how the weights spread (they differ by a few powers of two, and the counters of a histogram
-// would be hit by all lanes at once).  A trial costs two instructions a key and one exchange between the warps.  Lane-striped
-// slots (warp * 32 * KPT + i * 32 + lane) let a ballot count a row and keep every list in ascending order.
+// A team of CTAs - one, or a cluster of up to eight - settles a (sequence, kv head): which slots are kept, the ledger, and the list
+// of moves; a second launch moves the rows.  Order of keeping: protected tokens, then mass as a 32-bit key with the order of the
+// numbers.  The k-th largest key lies between two keys of the row; a trial in the middle counts those that reach it and finds
+// the nearest keys on either side of it, which become the new ends.  Nothing depends on how the weights spread (a histogram's
+// counters would be hit by all lanes at once: they differ by a few powers of two), and equal keys end the search.  Once few keys
+// are left between the ends, one warp settles those alone.  Lane-striped slots (warp * 32 * KPT + i * 32 + lane) let a ballot
+// count a row and keep every list in ascending order.
 struct EvictParams {
     Pages g;
     Batch q;
@@ -86,34 +87,93 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exchange of one number a warp; two buffers in turn, one barrier.
-struct CtaSum {
-    int* buf;      // [2][32]
-    int turn, warps;
-    __device__ __forceinline__ int all_of(int x) {         // what the lane's warp gave
-        int* b = buf + (turn & 1) * 32;
-        turn ^= 1;
-        const int lane = threadIdx.x & 31;
-        if (lane == 0) b[threadIdx.x >> 5] = x;
-        __syncthreads();
-        return lane < warps ? b[lane] : 0;
+constexpr int EV_KPT = 8, EV_WARPS = 16, EV_CTAS = 8;      // slots a thread, warps a CTA and CTAs a team at most
+constexpr int EV_FEW = 128;                                // keys that one warp settles alone
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void put_in_cta(uint32_t addr, const uint4& x) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+
+// Exchange of numbers between the warps of a team (TEAM: a cluster, else the CTA); two buffers in turn, one barrier.
+template <bool TEAM>
+struct Exchange {
+    uint4* buf;      // [2][EV_CTAS * EV_WARPS]
+    int turn, warps, ctas, rank;
+    __device__ __forceinline__ void sync() const {
+        if (!TEAM) {
+            __syncthreads();
+        } else {
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        }
     }
-    __device__ __forceinline__ int operator()(int x) { return __reduce_add_sync(0xffffffffu, all_of(x)); }
-    // the sum of the warps before this one, and of all
-    __device__ __forceinline__ int before(int x, int& total) {
-        const int y = all_of(x), lane = threadIdx.x & 31;
-        total = __reduce_add_sync(0xffffffffu, y);
-        return __reduce_add_sync(0xffffffffu, lane < (int)(threadIdx.x >> 5) ? y : 0);
+    __device__ __forceinline__ const uint4* give(uint4 x) {
+        uint4* b = buf + (turn & 1) * EV_CTAS * EV_WARPS;
+        turn ^= 1;
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        if (!TEAM) {
+            if (lane == 0) b[w] = x;
+        } else if (lane < ctas) {
+            put_in_cta(in_cta(tq_smem_u32(b + rank * warps + w), lane), x);
+        }
+        sync();
+        return b;
+    }
+    // every warp's numbers, one after the other: `take` is called with those of one or more warps a lane, or none
+    template <class F>
+    __device__ __forceinline__ void each(const uint4* b, F take) {
+        const int lane = threadIdx.x & 31;
+        if (!TEAM) {
+            if (lane < warps) take(b[lane], lane);
+        } else {
+            for (int j = lane; j < ctas * warps; j += 32) take(b[j], j);
+        }
+    }
+    // x: sum; y, z: largest
+    __device__ __forceinline__ uint4 trial(uint32_t x, uint32_t y, uint32_t z) {
+        const uint4* b = give(make_uint4(__reduce_add_sync(0xffffffffu, x), __reduce_max_sync(0xffffffffu, y), __reduce_max_sync(0xffffffffu, z), 0u));
+        uint32_t s = 0, t = 0, u = 0;
+        each(b, [&](const uint4& v, int) { s += v.x, t = max(t, v.y), u = max(u, v.z); });
+        return make_uint4(__reduce_add_sync(0xffffffffu, s), __reduce_max_sync(0xffffffffu, t), __reduce_max_sync(0xffffffffu, u), 0u);
+    }
+    // sums of two numbers a warp over the warps before this one (x, y) and over all (z, w)
+    __device__ __forceinline__ uint4 before(uint32_t x, uint32_t y) {
+        const uint4* b = give(make_uint4(x, y, 0u, 0u));
+        const int me = rank * warps + (int)(threadIdx.x >> 5);
+        uint32_t s = 0, t = 0, ps = 0, pt = 0;
+        each(b, [&](const uint4& v, int j) {
+            s += v.x, t += v.y;
+            if (j < me) ps += v.x, pt += v.y;
+        });
+        return make_uint4(__reduce_add_sync(0xffffffffu, ps), __reduce_add_sync(0xffffffffu, pt), __reduce_add_sync(0xffffffffu, s),
+                          __reduce_add_sync(0xffffffffu, t));
     }
 };
 
-// KPT slots a thread, held as keys in registers; a row that is longer than all threads hold (LONG) is gone over again for every
+// A thread holds EV_KPT slots as keys in registers; a row that is longer than the team holds (LONG) is gone over again for every
 // count.  Masses and positions are read again where they are written: they are in the caches.
-template <int KPT, bool LONG>
-__global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams p) {
-    __shared__ int s_buf[64];
-    const int row = blockIdx.x, b = row / p.g.H, lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+template <bool TEAM, bool LONG>
+__global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
+    constexpr int KPT = EV_KPT;
+    __shared__ uint4 s_buf[2 * EV_CTAS * EV_WARPS];
+    __shared__ uint32_t s_few[EV_FEW], s_count;            // of the first CTA: the keys left, their number
+    __shared__ uint4 s_found;                              // the limit, and how many equal to it are taken
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t below = (1u << lane) - 1u;
+    int ctas = 1, rank = 0;
+    if (TEAM) {
+        asm("mov.u32 %0, %cluster_nctarank;" : "=r"(ctas));
+        asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+    }
+    const int row = blockIdx.x / ctas, b = row / p.g.H;
+    Exchange<TEAM> team{s_buf, 0, warps, ctas, rank};
+    if (threadIdx.x == 0) s_count = 0;
+    if (TEAM) team.sync();                             // the others have begun: their shared memory may be written
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = seq_len(p.q, b, p.status), m = min(n, p.budget);
@@ -123,31 +183,26 @@ __global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams 
     float* out_mass = p.out_mass + row * p.out_stride;
     int32_t* out_positions = p.out_positions + row * p.out_stride;
     int32_t *dst = p.dst + (int64_t)row * p.list, *src = p.src + (int64_t)row * p.list;
-    CtaSum sum{s_buf, 0, warps};
-    const int span = warps * 32 * KPT, rounds = LONG ? (n + span - 1) / span : 1;
+    const int span = ctas * warps * 32 * KPT, rounds = LONG ? (n + span - 1) / span : 1;
 
     uint32_t key[KPT];                 // 0: not in the cache
     uint32_t guard = 0;                // bit i: slot i of this thread is protected
-    auto slot_of = [&](int r, int i) { return r * span + (w * KPT + i) * 32 + lane; };
+    auto first_slot = [&](int r) { return r * span + (rank * warps + w) * 32 * KPT + lane; };
     auto position = [&](int t) { return t < held ? positions[t] : seen + t - held; };
     auto load = [&](int r) {
-        const int t0 = slot_of(r, 0);
+        const int t0 = first_slot(r);
+        float x[KPT];
+        int pos[KPT];
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) x[i] = t0 + i * 32 < n ? mass[t0 + i * 32] : 0.f;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) pos[i] = t0 + i * 32 < n ? position(t0 + i * 32) : 0;
         guard = 0;
 #pragma unroll
-        for (int c = 0; c < KPT; c += 8) {                 // eight at a time: more would not fit the registers
-            float x[8];
-            int pos[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = t0 + (c + i) * 32 < n ? mass[t0 + (c + i) * 32] : 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pos[i] = t0 + (c + i) * 32 < n ? position(t0 + (c + i) * 32) : 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool there = t0 + (c + i) * 32 < n;
-                key[c + i] = there ? key_of(x[i]) : 0u;
-                guard |= (uint32_t)(there && pos[i] >= late) << (c + i);
-            }
-            asm volatile("" ::: "memory");
+        for (int i = 0; i < KPT; ++i) {
+            const bool there = t0 + i * 32 < n;
+            key[i] = there ? key_of(x[i]) : 0u;
+            guard |= (uint32_t)(there && pos[i] >= late) << i;
         }
     };
     load(0);
@@ -158,68 +213,101 @@ __global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams 
     uint32_t limit = 0u;               // the k-th largest key of the candidates
     int equal_taken = 0;               // how many of the keys equal to it are taken, lowest slots first
     auto among = [&](int i) { return ((guard >> i) & 1u) == (uint32_t)all_guarded; };
+    auto drop = [&]() {                // keys of others than candidates are 0, and no trial value is
+#pragma unroll
+        for (int i = 0; i < KPT; ++i)
+            if (!among(i)) key[i] = 0u;
+    };
     if (trims) {
         int guarded = 0;
         for (int r = 0; r < rounds; ++r) {
             if (LONG && r > 0) load(r);
             guarded += __popc(guard);
         }
-        guarded = sum(__reduce_add_sync(0xffffffffu, guarded));
+        guarded = (int)team.trial((uint32_t)guarded, 0u, 0u).x;
         all_guarded = guarded >= m;
         const int k = all_guarded ? m : m - guarded;
-        // keys of others than candidates are 0 from here on, and no trial value is
-        uint32_t ones = 0xffffffffu, any = 0u;
-        auto drop = [&]() {
-#pragma unroll
-            for (int i = 0; i < KPT; ++i)
-                if (!among(i)) key[i] = 0u;
-        };
+        uint32_t low = 0u, high = 0u;                      // of the candidates' keys: the largest complement, the largest
         for (int r = 0; r < rounds; ++r) {
             if (LONG) load(r);
             drop();
 #pragma unroll
             for (int i = 0; i < KPT; ++i)
-                if (key[i] != 0u) ones &= key[i], any |= key[i];
+                if (key[i] != 0u) low = max(low, ~key[i]), high = max(high, key[i]);
         }
-        ones = (uint32_t)sum.all_of((int)__reduce_and_sync(0xffffffffu, ones));
-        any = (uint32_t)sum.all_of((int)__reduce_or_sync(0xffffffffu, any));
-        ones = __reduce_and_sync(0xffffffffu, lane < warps ? ones : 0xffffffffu);
-        any = __reduce_or_sync(0xffffffffu, any);
-        const uint32_t differ = ones ^ any;
-        int bit = 31 - __clz(differ), reach = -1;          // reach: keys >= limit
-        limit = differ == 0u ? any : bit == 31 ? 0u : any >> (bit + 1) << (bit + 1);       // what all candidates have in common
-        for (; bit >= 0 && reach != k; --bit) {
-            const uint32_t trial = limit | (1u << bit);
+        // the k-th largest lies from lo to hi, both keys of the row: `reach` keys are >= lo, `above` > hi
+        const uint4 ends = team.trial(0u, low, high);
+        uint32_t lo = ~ends.y, hi = ends.z;
+        int reach = all_guarded ? guarded : n - guarded, above = 0;
+        while (k > 0 && lo < hi && reach != k && reach - above > EV_FEW) {
+            const uint32_t trial = lo + (hi - lo) / 2 + 1;
             int c = 0;
+            uint32_t under = 0u, over = 0u;                // the largest key below the trial, the complement of the least that reaches it
             for (int r = 0; r < rounds; ++r) {
                 if (LONG) {
                     load(r);
                     drop();
                 }
 #pragma unroll
-                for (int i = 0; i < KPT; ++i) c += key[i] >= trial;
+                for (int i = 0; i < KPT; ++i) {
+                    const bool there = key[i] >= trial;
+                    c += there;
+                    if (there) over = max(over, ~key[i]);
+                    else under = max(under, key[i]);
+                }
             }
-            c = sum(__reduce_add_sync(0xffffffffu, c));
-            if (c >= k) {
-                limit = trial;
-                reach = c;
-            }
+            const uint4 got = team.trial((uint32_t)c, under, over);
+            if ((int)got.x >= k) lo = ~got.z, reach = (int)got.x;
+            else hi = got.y, above = (int)got.x;
         }
         if (k == 0) {                                      // nothing but the protected ones
             limit = 0xffffffffu;
-        } else if (reach == k) {
-            equal_taken = 0x7fffffff;
+        } else if (reach == k || lo == hi) {
+            limit = lo;
+            equal_taken = reach == k ? 0x7fffffff : k - above;
         } else {
-            int above = 0;
+            // the keys from lo to hi, few enough for one warp, go to the first CTA
+            const uint32_t count_at = in_cta(tq_smem_u32(&s_count), 0), few_at = in_cta(tq_smem_u32(s_few), 0);
             for (int r = 0; r < rounds; ++r) {
                 if (LONG) {
                     load(r);
                     drop();
                 }
 #pragma unroll
-                for (int i = 0; i < KPT; ++i) above += key[i] > limit;
+                for (int i = 0; i < KPT; ++i)
+                    if (key[i] >= lo && key[i] <= hi) {
+                        uint32_t at;
+                        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at) : "memory");
+                        if (at < EV_FEW) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(few_at + at * 4), "r"(key[i]) : "memory");
+                    }
             }
-            equal_taken = k - sum(__reduce_add_sync(0xffffffffu, above));
+            team.sync();
+            if (rank == 0 && w == 0) {
+                uint32_t mine[EV_FEW / 32];
+#pragma unroll
+                for (int i = 0; i < EV_FEW / 32; ++i) mine[i] = i * 32 + lane < (int)s_count ? s_few[i * 32 + lane] : 0u;
+                const int want = k - above;
+                int there = reach - above, over = 0;       // of the few: >= lo, > hi
+                while (lo < hi && there != want) {
+                    const uint32_t trial = lo + (hi - lo) / 2 + 1;
+                    int c = 0;
+                    uint32_t under = 0u, least = 0u;
+#pragma unroll
+                    for (int i = 0; i < EV_FEW / 32; ++i) {
+                        c += mine[i] >= trial;
+                        if (mine[i] >= trial) least = max(least, ~mine[i]);
+                        else under = max(under, mine[i]);
+                    }
+                    c = (int)__reduce_add_sync(0xffffffffu, c);
+                    if (c >= want) lo = ~__reduce_max_sync(0xffffffffu, least), there = c;
+                    else hi = __reduce_max_sync(0xffffffffu, under), over = c;
+                }
+                const uint4 found = make_uint4(lo, there == want ? 0x7fffffffu : (uint32_t)(want - over), 0u, 0u);
+                if (lane < ctas) put_in_cta(in_cta(tq_smem_u32(&s_found), lane), found);
+            }
+            team.sync();
+            limit = s_found.x;
+            equal_taken = (int)s_found.y;
         }
     }
 
@@ -228,20 +316,18 @@ __global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams 
     for (int r = 0; r < rounds; ++r) {
         if (LONG) {
             load(r);
-            if (trims) {
-#pragma unroll
-                for (int i = 0; i < KPT; ++i)
-                    if (!among(i)) key[i] = 0u;
-            }
+            if (trims) drop();
         }
-        const int t0 = slot_of(r, 0);
-        int mine = 0, total;
-        if (trims) {
+        const int t0 = first_slot(r);
+        int rank_eq = 0;
+        if (trims && equal_taken != 0x7fffffff) {          // ranks of the keys equal to the limit, where not all are taken
+            int mine = 0;
 #pragma unroll
             for (int i = 0; i < KPT; ++i) mine += __popc(__ballot_sync(0xffffffffu, key[i] != 0u && key[i] == limit));
+            const uint4 at = team.before((uint32_t)mine, 0u);
+            rank_eq = equals + (int)at.x;
+            equals += (int)at.z;
         }
-        int rank = equals + sum.before(mine, total);
-        equals += total;
         uint32_t kept = 0;                                 // bit i: slot i of this thread stays in the cache
         int my_holes = 0, my_movers = 0;
 #pragma unroll
@@ -250,50 +336,59 @@ __global__ void __launch_bounds__(1024) tq_pages_evict_kernel(const EvictParams 
             bool stays = t < n;
             if (trims) {
                 const uint32_t eq = __ballot_sync(0xffffffffu, key[i] != 0u && key[i] == limit);
-                stays = stays && (among(i) ? key[i] > limit || (key[i] == limit && rank + __popc(eq & below) < equal_taken) : !all_guarded);
-                rank += __popc(eq);
+                stays = stays && (among(i) ? key[i] > limit || (key[i] == limit && rank_eq + __popc(eq & below) < equal_taken) : !all_guarded);
+                rank_eq += __popc(eq);
             }
             my_holes += __popc(__ballot_sync(0xffffffffu, t < m && !stays));
             my_movers += __popc(__ballot_sync(0xffffffffu, t >= m && stays));
             kept |= (uint32_t)stays << i;
         }
-        int total_holes, total_movers;
-        int hole_at = holes + sum.before(my_holes, total_holes), mover_at = movers + sum.before(my_movers, total_movers);
-        holes += total_holes;
-        movers += total_movers;
+        int hole_at = 0, mover_at = 0;
+        if (trims) {
+            const uint4 at = team.before((uint32_t)my_holes, (uint32_t)my_movers);
+            hole_at = holes + (int)at.x, mover_at = movers + (int)at.y;
+            holes += (int)at.z, movers += (int)at.w;
+        }
+        // all loads in front of the first store: the arrays may be the same ones
+        float x[KPT];
+        int pos[KPT];
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int t = t0 + i * 32;
+            if ((kept >> i) & 1) x[i] = mass[t], pos[i] = position(t);
+        }
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const int t = t0 + i * 32;
             const bool stays = (kept >> i) & 1;
-            const uint32_t hole = __ballot_sync(0xffffffffu, t < m && !stays);
-            if (t < m && !stays) dst[hole_at + __popc(hole & below)] = t;
-            hole_at += __popc(hole);
-            if (t < m && stays) {
-                out_mass[t] = mass[t];
-                out_positions[t] = position(t);
+            if (trims) {
+                const uint32_t hole = __ballot_sync(0xffffffffu, t < m && !stays);
+                if (t < m && !stays) dst[hole_at + __popc(hole & below)] = t;
+                hole_at += __popc(hole);
             }
+            if (t < m && stays) out_mass[t] = x[i], out_positions[t] = pos[i];
         }
-        __syncthreads();                                   // every hole that a mover of this round takes has been noted: holes lie before movers
+        if (!trims) continue;
+        team.sync();                                       // every hole that a mover of this round takes has been noted: holes lie before movers
+        int at[KPT], to[KPT];
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            const int t = t0 + i * 32;
-            const bool moves = t >= m && ((kept >> i) & 1);
+            const bool moves = t0 + i * 32 >= m && ((kept >> i) & 1);
             const uint32_t mover = __ballot_sync(0xffffffffu, moves);
-            if (moves) {
-                const int j = mover_at + __popc(mover & below), to = dst[j];
-                src[j] = t;
-                out_mass[to] = mass[t];
-                out_positions[to] = position(t);
-            }
+            at[i] = moves ? mover_at + __popc(mover & below) : -1;
             mover_at += __popc(mover);
+            if (moves) to[i] = __ldcg(dst + at[i]);
         }
+#pragma unroll
+        for (int i = 0; i < KPT; ++i)
+            if (at[i] >= 0) src[at[i]] = t0 + i * 32, out_mass[to[i]] = x[i], out_positions[to[i]] = pos[i];
     }
-    __syncthreads();                                       // in place: nothing is cleared before it has been read
-    for (int64_t t = m + (int)threadIdx.x; t < p.out_stride; t += blockDim.x) {
+    team.sync();                                           // in place: nothing is cleared before it has been read
+    for (int64_t t = m + rank * (int)blockDim.x + (int)threadIdx.x; t < p.out_stride; t += ctas * blockDim.x) {
         out_mass[t] = 0.f;
         out_positions[t] = -1;
     }
-    if (threadIdx.x == 0) p.count[row] = holes;
+    if (rank == 0 && threadIdx.x == 0) p.count[row] = holes;
 }
 
 // The moves of all (sequence, kv head) rows: a group of D/8 lanes copies a key row, then a value row.
@@ -410,13 +505,15 @@ extern "C" int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     tq_note_launch(st, TQ_LAUNCH_WAITED);      // writes rows that a store may read next
-    const int n = batch->max_seq_len;
-    auto threads_for = [&](int kpt) { return n >= 1024 * kpt ? 1024 : (n + 32 * kpt - 1) / (32 * kpt) * 32; };
-    int rc2;
-    // eight keys a thread as far as 1024 threads hold the row, then thirty-two
-    if (n <= 1024 * 8) rc2 = launch_behind(tq_pages_evict_kernel<8, false>, dim3((unsigned)rows), threads_for(8), 0, st, p);
-    else if (n <= 1024 * 32) rc2 = launch_behind(tq_pages_evict_kernel<32, false>, dim3((unsigned)rows), threads_for(32), 0, st, p);
-    else rc2 = launch_behind(tq_pages_evict_kernel<32, true>, dim3((unsigned)rows), 1024, 0, st, p);
+    // as many CTAs a row as it takes to hold its keys in registers, up to eight; no more warps than hold them
+    const int n = batch->max_seq_len, cta = EV_WARPS * 32 * EV_KPT;
+    const int ctas = n <= cta ? 1 : n <= 2 * cta ? 2 : n <= 4 * cta ? 4 : EV_CTAS;
+    const int each = (n + ctas - 1) / ctas, threads = each >= cta ? EV_WARPS * 32 : (each + 32 * EV_KPT - 1) / (32 * EV_KPT) * 32;
+    if (rows * ctas >= ((int64_t)1 << 31)) return TQ_ERR_SHAPE;
+    const dim3 teams((unsigned)(rows * ctas));
+    const int rc2 = ctas == 1 ? launch_behind(tq_pages_evict_kernel<false, false>, teams, threads, 0, st, p)
+                    : n <= ctas * cta ? launch_behind_in_clusters(tq_pages_evict_kernel<true, false>, teams, threads, ctas, st, p)
+                                      : launch_behind_in_clusters(tq_pages_evict_kernel<true, true>, teams, threads, ctas, st, p);
     if (rc2 != TQ_OK) return rc2;
     const int per = 256 / (pages->head_dim / 8);
     const int64_t tiles = (p.list + per - 1) / per;
