@@ -317,7 +317,8 @@ def same_bits(a, b):
 @pytest.mark.parametrize("lens,budget,recent,D,H,page,slots", [
     ([300], 256, 32, 128, 2, 16, 300), ([40, 0, 5, 64, 65], 64, 64, 64, 3, 7, 70), ([100, 90], 1, 1, 128, 1, 16, 128),
     ([100, 3], 0, 0, 128, 2, 16, 100), ([33, 2048, 2049, 1500], 1000, 0, 64, 1, 16, 2049), ([5000, 8192], 700, 100, 64, 1, 32, 8192),
-    ([8193, 9000, 20], 4096, 300, 64, 1, 16, 9001), ([20011], 19000, 19000, 64, 1, 64, 20011), ([50, 60], 500, 20, 256, 2, 24, 60),
+    ([8193, 9000, 20], 4096, 300, 64, 1, 16, 9001), ([20011], 19000, 19000, 64, 1, 64, 20011), ([40000, 1500], 1000, 64, 64, 1, 128, 40000),
+    ([70001], 3000, 100, 64, 1, 128, 70100), ([50, 60], 500, 20, 256, 2, 24, 60),
 ])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_evict(lens, budget, recent, D, H, page, slots, in_place):

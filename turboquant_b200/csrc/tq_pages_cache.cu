@@ -87,8 +87,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int EV_KPT = 8, EV_WARPS = 16, EV_CTAS = 8;      // slots a thread, warps a CTA and CTAs a team at most
-constexpr int EV_FEW = 128;                                // keys that one warp settles alone
+constexpr int EV_KPT = 8, EV_WARPS = 32, EV_CTAS = 8;      // slots a thread, warps a CTA and CTAs a team at most
+constexpr int EV_SOME = EV_WARPS * 32 * EV_KPT, EV_FEW = 128;      // keys that a team's first CTA, and that one warp settles alone
 
 __device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
     uint32_t r;
@@ -99,11 +99,12 @@ __device__ __forceinline__ void put_in_cta(uint32_t addr, const uint4& x) {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
-// Exchange of numbers between the warps of a team (TEAM: a cluster, else the CTA); two buffers in turn, one barrier.
+// Exchange of numbers between the warps of a CTA and, in a TEAM, between the CTAs of a cluster: two buffers in turn each, a
+// barrier of each kind (the cluster's takes over a microsecond).
 template <bool TEAM>
 struct Exchange {
-    uint4* buf;      // [2][EV_CTAS * EV_WARPS]
-    int turn, warps, ctas, rank;
+    uint4* buf;      // [2][EV_WARPS], then [2][EV_CTAS]
+    int turn, turn_team, warps, ctas, rank;
     __device__ __forceinline__ void sync() const {
         if (!TEAM) {
             __syncthreads();
@@ -113,45 +114,45 @@ struct Exchange {
         }
     }
     __device__ __forceinline__ const uint4* give(uint4 x) {
-        uint4* b = buf + (turn & 1) * EV_CTAS * EV_WARPS;
+        uint4* b = buf + turn * EV_WARPS;
         turn ^= 1;
-        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-        if (!TEAM) {
-            if (lane == 0) b[w] = x;
-        } else if (lane < ctas) {
-            put_in_cta(in_cta(tq_smem_u32(b + rank * warps + w), lane), x);
-        }
+        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = x;
+        __syncthreads();
+        return b;
+    }
+    // the CTA's number, the same in every warp, to all CTAs
+    __device__ __forceinline__ const uint4* give_team(uint4 x) {
+        uint4* b = buf + 2 * EV_WARPS + turn_team * EV_CTAS;
+        turn_team ^= 1;
+        if ((int)threadIdx.x < ctas) put_in_cta(in_cta(tq_smem_u32(b + rank), (int)threadIdx.x), x);
         sync();
         return b;
     }
-    // every warp's numbers, one after the other: `take` is called with those of one or more warps a lane, or none
-    template <class F>
-    __device__ __forceinline__ void each(const uint4* b, F take) {
+    __device__ __forceinline__ uint4 join(const uint4* b, int n) const {
         const int lane = threadIdx.x & 31;
-        if (!TEAM) {
-            if (lane < warps) take(b[lane], lane);
-        } else {
-            for (int j = lane; j < ctas * warps; j += 32) take(b[j], j);
-        }
+        const uint4 v = lane < n ? b[lane] : make_uint4(0u, 0u, 0u, 0u);
+        return make_uint4(__reduce_add_sync(0xffffffffu, v.x), __reduce_max_sync(0xffffffffu, v.y), __reduce_max_sync(0xffffffffu, v.z), 0u);
     }
-    // x: sum; y, z: largest
-    __device__ __forceinline__ uint4 trial(uint32_t x, uint32_t y, uint32_t z) {
-        const uint4* b = give(make_uint4(__reduce_add_sync(0xffffffffu, x), __reduce_max_sync(0xffffffffu, y), __reduce_max_sync(0xffffffffu, z), 0u));
-        uint32_t s = 0, t = 0, u = 0;
-        each(b, [&](const uint4& v, int) { s += v.x, t = max(t, v.y), u = max(u, v.z); });
-        return make_uint4(__reduce_add_sync(0xffffffffu, s), __reduce_max_sync(0xffffffffu, t), __reduce_max_sync(0xffffffffu, u), 0u);
+    // x: sum; y, z: largest.  `alone`: within this CTA
+    __device__ __forceinline__ uint4 trial(uint32_t x, uint32_t y, uint32_t z, bool alone = false) {
+        uint4 r = join(give(make_uint4(__reduce_add_sync(0xffffffffu, x), __reduce_max_sync(0xffffffffu, y), __reduce_max_sync(0xffffffffu, z), 0u)), warps);
+        if (TEAM && !alone) r = join(give_team(r), ctas);
+        return r;
     }
     // sums of two numbers a warp over the warps before this one (x, y) and over all (z, w)
     __device__ __forceinline__ uint4 before(uint32_t x, uint32_t y) {
-        const uint4* b = give(make_uint4(x, y, 0u, 0u));
-        const int me = rank * warps + (int)(threadIdx.x >> 5);
-        uint32_t s = 0, t = 0, ps = 0, pt = 0;
-        each(b, [&](const uint4& v, int j) {
-            s += v.x, t += v.y;
-            if (j < me) ps += v.x, pt += v.y;
-        });
-        return make_uint4(__reduce_add_sync(0xffffffffu, ps), __reduce_add_sync(0xffffffffu, pt), __reduce_add_sync(0xffffffffu, s),
-                          __reduce_add_sync(0xffffffffu, t));
+        const int lane = threadIdx.x & 31;
+        auto add = [&](const uint4* b, int n, int me) {
+            const uint4 v = lane < n ? b[lane] : make_uint4(0u, 0u, 0u, 0u);
+            return make_uint4(__reduce_add_sync(0xffffffffu, lane < me ? v.x : 0u), __reduce_add_sync(0xffffffffu, lane < me ? v.y : 0u),
+                              __reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y));
+        };
+        uint4 r = add(give(make_uint4(x, y, 0u, 0u)), warps, (int)(threadIdx.x >> 5));
+        if (TEAM) {
+            const uint4 t = add(give_team(make_uint4(r.z, r.w, 0u, 0u)), ctas, rank);
+            r = make_uint4(r.x + t.x, r.y + t.y, t.z, t.w);
+        }
+        return r;
     }
 };
 
@@ -160,8 +161,9 @@ struct Exchange {
 template <bool TEAM, bool LONG>
 __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
     constexpr int KPT = EV_KPT;
-    __shared__ uint4 s_buf[2 * EV_CTAS * EV_WARPS];
-    __shared__ uint32_t s_few[EV_FEW], s_count;            // of the first CTA: the keys left, their number
+    __shared__ uint4 s_buf[2 * EV_WARPS + 2 * EV_CTAS];
+    __shared__ uint32_t s_some[TEAM ? EV_SOME : 1];        // of a team's first CTA: the keys left for it
+    __shared__ uint32_t s_few[EV_FEW], s_count[2];         // the keys left for one warp; their numbers
     __shared__ uint4 s_found;                              // the limit, and how many equal to it are taken
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t below = (1u << lane) - 1u;
@@ -171,8 +173,8 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
         asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
     }
     const int row = blockIdx.x / ctas, b = row / p.g.H;
-    Exchange<TEAM> team{s_buf, 0, warps, ctas, rank};
-    if (threadIdx.x == 0) s_count = 0;
+    Exchange<TEAM> team{s_buf, 0, 0, warps, ctas, rank};
+    if (threadIdx.x < 2) s_count[threadIdx.x] = 0;
     if (TEAM) team.sync();                             // the others have begun: their shared memory may be written
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -220,41 +222,54 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
     };
     if (trims) {
         int guarded = 0;
+        uint32_t low = 0u, high = 0u;                      // of the candidates' keys: the largest complement, the largest
+        auto ends_of = [&]() {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)
+                if (key[i] != 0u && among(i)) low = max(low, ~key[i]), high = max(high, key[i]);
+        };
         for (int r = 0; r < rounds; ++r) {
             if (LONG && r > 0) load(r);
             guarded += __popc(guard);
+            ends_of();
         }
-        guarded = (int)team.trial((uint32_t)guarded, 0u, 0u).x;
-        all_guarded = guarded >= m;
+        uint4 ends = team.trial((uint32_t)guarded, low, high);
+        guarded = (int)ends.x;
+        if (guarded >= m) {                                // the protected ones alone are too many
+            all_guarded = true;
+            low = high = 0u;
+            for (int r = 0; r < rounds; ++r) {
+                if (LONG) load(r);
+                ends_of();
+            }
+            ends = team.trial(0u, low, high);
+        }
         const int k = all_guarded ? m : m - guarded;
-        uint32_t low = 0u, high = 0u;                      // of the candidates' keys: the largest complement, the largest
-        for (int r = 0; r < rounds; ++r) {
-            if (LONG) load(r);
-            drop();
-#pragma unroll
-            for (int i = 0; i < KPT; ++i)
-                if (key[i] != 0u) low = max(low, ~key[i]), high = max(high, key[i]);
-        }
+        drop();
         // the k-th largest lies from lo to hi, both keys of the row: `reach` keys are >= lo, `above` > hi
-        const uint4 ends = team.trial(0u, low, high);
         uint32_t lo = ~ends.y, hi = ends.z;
         int reach = all_guarded ? guarded : n - guarded, above = 0;
-        while (k > 0 && lo < hi && reach != k && reach - above > EV_FEW) {
+        // a trial: the keys that reach it, the largest below it, the complement of the least that reaches it
+        auto count = [&](uint32_t trial, int& c, uint32_t& under, uint32_t& over) {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                const bool there = key[i] >= trial;
+                c += there;
+                if (there) over = max(over, ~key[i]);
+                else under = max(under, key[i]);
+            }
+        };
+        const int few = TEAM ? (int)blockDim.x * KPT : EV_FEW;
+        while (k > 0 && lo < hi && reach != k && reach - above > few) {
             const uint32_t trial = lo + (hi - lo) / 2 + 1;
             int c = 0;
-            uint32_t under = 0u, over = 0u;                // the largest key below the trial, the complement of the least that reaches it
+            uint32_t under = 0u, over = 0u;
             for (int r = 0; r < rounds; ++r) {
                 if (LONG) {
                     load(r);
                     drop();
                 }
-#pragma unroll
-                for (int i = 0; i < KPT; ++i) {
-                    const bool there = key[i] >= trial;
-                    c += there;
-                    if (there) over = max(over, ~key[i]);
-                    else under = max(under, key[i]);
-                }
+                count(trial, c, under, over);
             }
             const uint4 got = team.trial((uint32_t)c, under, over);
             if ((int)got.x >= k) lo = ~got.z, reach = (int)got.x;
@@ -266,26 +281,66 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
             limit = lo;
             equal_taken = reach == k ? 0x7fffffff : k - above;
         } else {
-            // the keys from lo to hi, few enough for one warp, go to the first CTA
-            const uint32_t count_at = in_cta(tq_smem_u32(&s_count), 0), few_at = in_cta(tq_smem_u32(s_few), 0);
-            for (int r = 0; r < rounds; ++r) {
-                if (LONG) {
-                    load(r);
-                    drop();
-                }
+            // the keys from lo to hi go to fewer hands: those of a team to its first CTA, whose go on, and those to one warp
+            auto collect = [&](uint32_t* list, uint32_t* number, int most) {
+                const uint32_t count_at = in_cta(tq_smem_u32(number), 0), list_at = in_cta(tq_smem_u32(list), 0);
 #pragma unroll
                 for (int i = 0; i < KPT; ++i)
                     if (key[i] >= lo && key[i] <= hi) {
                         uint32_t at;
                         asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at) : "memory");
-                        if (at < EV_FEW) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(few_at + at * 4), "r"(key[i]) : "memory");
+                        if (at < (uint32_t)most) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(list_at + at * 4), "r"(key[i]) : "memory");
                     }
+            };
+            if (TEAM) {
+                for (int r = 0; r < rounds; ++r) {
+                    if (LONG) {
+                        load(r);
+                        drop();
+                    }
+                    collect(s_some, s_count, EV_SOME);
+                }
+                team.sync();
             }
-            team.sync();
+            bool settled = false;
+            if (!TEAM || rank == 0) {
+                uint32_t held_keys[KPT];                   // a team's first CTA: its own keys make room for those left
+                if (TEAM) {
+#pragma unroll
+                    for (int i = 0; i < KPT; ++i) {
+                        held_keys[i] = key[i];
+                        const int j = i * (int)blockDim.x + (int)threadIdx.x;
+                        key[i] = j < (int)s_count[0] ? s_some[j] : 0u;
+                    }
+                    // of them: `above` lie over hi
+                    const int want = k - above;
+                    int there = reach - above, over_hi = 0;
+                    while (lo < hi && there != want && there - over_hi > EV_FEW) {
+                        const uint32_t trial = lo + (hi - lo) / 2 + 1;
+                        int c = 0;
+                        uint32_t under = 0u, over = 0u;
+                        count(trial, c, under, over);
+                        const uint4 got = team.trial((uint32_t)c, under, over, true);
+                        if ((int)got.x >= want) lo = ~got.z, there = (int)got.x;
+                        else hi = got.y, over_hi = (int)got.x;
+                    }
+                    reach = there + above;
+                    above += over_hi;
+                    settled = lo == hi || reach == k;
+                }
+                if (!settled) {
+                    collect(s_few, s_count + 1, EV_FEW);
+                    __syncthreads();
+                }
+                if (TEAM) {
+#pragma unroll
+                    for (int i = 0; i < KPT; ++i) key[i] = held_keys[i];
+                }
+            }
             if (rank == 0 && w == 0) {
                 uint32_t mine[EV_FEW / 32];
 #pragma unroll
-                for (int i = 0; i < EV_FEW / 32; ++i) mine[i] = i * 32 + lane < (int)s_count ? s_few[i * 32 + lane] : 0u;
+                for (int i = 0; i < EV_FEW / 32; ++i) mine[i] = !settled && i * 32 + lane < (int)s_count[1] ? s_few[i * 32 + lane] : 0u;
                 const int want = k - above;
                 int there = reach - above, over = 0;       // of the few: >= lo, > hi
                 while (lo < hi && there != want) {
@@ -343,12 +398,6 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
             my_movers += __popc(__ballot_sync(0xffffffffu, t >= m && stays));
             kept |= (uint32_t)stays << i;
         }
-        int hole_at = 0, mover_at = 0;
-        if (trims) {
-            const uint4 at = team.before((uint32_t)my_holes, (uint32_t)my_movers);
-            hole_at = holes + (int)at.x, mover_at = movers + (int)at.y;
-            holes += (int)at.z, movers += (int)at.w;
-        }
         // all loads in front of the first store: the arrays may be the same ones
         float x[KPT];
         int pos[KPT];
@@ -356,6 +405,12 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
         for (int i = 0; i < KPT; ++i) {
             const int t = t0 + i * 32;
             if ((kept >> i) & 1) x[i] = mass[t], pos[i] = position(t);
+        }
+        int hole_at = 0, mover_at = 0;
+        if (trims) {
+            const uint4 at = team.before((uint32_t)my_holes, (uint32_t)my_movers);
+            hole_at = holes + (int)at.x, mover_at = movers + (int)at.y;
+            holes += (int)at.z, movers += (int)at.w;
         }
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
