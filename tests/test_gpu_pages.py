@@ -517,6 +517,108 @@ def test_a_prompt_evicted_then_compressed():
     assert torch.equal(compute_hybrid_attention(q.cuda(), a, None, None, H * G), compute_hybrid_attention(q.cuda(), b, None, None, H * G))
 
 
+def test_more_sequences_than_a_cta_has_threads():
+    """Lengths are looked at 256 at a time; every third sequence is empty."""
+    rng = random.Random(3)
+    lens = [0 if i % 3 == 0 else rng.randint(1, 70) for i in range(700)]
+    s = Setup(lens, 2, 64, 16, FP16, seed=30)
+    led, led2 = AttentionLedger(700, 2, s.longest, "cuda"), AttentionLedger(700, 2, s.longest, "cuda")
+    q, win = s.query(700, heads=4), s.query(700, 3, heads=4)
+    out = s.cache.decode(q.cuda(), s.dtable, s.dlens, s.longest, ledger=led).cpu().double()
+    s.cache.observe(win.cuda(), s.dtable, s.dlens, s.longest, led2)
+    for b in range(0, 700):
+        k, v = s.rows(b)
+        qb = q[b].double().view(1, 2, 2, 64)
+        ref, p = O.attention(qb, k, v)
+        rel = weight_error(qb, k, 64 ** -0.5)
+        check_out(out[b].view(1, 2, 2, 64), ref, p, v, FP16, rel)
+        if lens[b]:
+            _, pw = O.attention(win[b].double().view(3, 2, 2, 64), k, v, last=torch.arange(lens[b] - 3, lens[b]))
+            for m, add in ((led.mass, p[0].sum(1)), (led2.mass, pw.sum((0, 2)))):
+                assert ((m[b, :, :lens[b]].cpu().double() - add).abs() <= add * (rel + 2.0 ** -20)).all()
+    for m in (led, led2):
+        m.mass.copy_(torch.rand(m.mass.shape, generator=s.gen))
+    want = _evict_reference(s, led, lens, 20, 5)
+    got = s.cache.evict(s.dtable, s.dlens, s.longest, led, 20, 5)
+    assert got.tolist() == want[4] and same_bits(led.mass, want[2]) and same_bits(s.cache.key_cache, want[0]) and s.cache.status() == 0
+
+
+def test_planes_beyond_four_gigabytes():
+    """Pages at the end of planes of 2^32 bytes and more each: every kernel's offsets pass 32 bits."""
+    H, D, page = 8, 128, 16
+    blocks = (2 ** 32 + 2 ** 27) // (page * H * D * 2)
+    planes = torch.zeros(2, blocks, page, H, D, dtype=BF16, device="cuda")
+    cache = PagedKVCache(ExactCacheSpec(D, H), planes[0], planes[1])
+    n, g = 100, torch.Generator().manual_seed(2)
+    table = torch.arange(blocks - 7, blocks, dtype=torch.int32, device="cuda").flip(0).view(1, 7)
+    t = torch.arange(n, device="cuda")
+    k, v = (torch.randn(n, H, D, generator=g).to(BF16) for _ in range(2))
+    cache.write(k.cuda(), v.cuda(), table[0, t // page].long() * page + t % page)
+    lens, led, led2 = torch.tensor([n], dtype=torch.int32, device="cuda"), AttentionLedger(1, H, n, "cuda"), AttentionLedger(1, H, n, "cuda")
+    q = torch.randn(1, 4 * H, D, generator=g).to(BF16)
+    out = cache.decode(q.cuda(), table, lens, n, ledger=led)
+    cache.observe(q[:, None].cuda(), table, lens, n, led2)
+    ref, p = O.attention(q[0].double().view(1, H, 4, D), k.double(), v.double())
+    rel = weight_error(q.double(), k.double(), D ** -0.5)
+    check_out(out.cpu().double().view(1, H, 4, D), ref, p, v.double(), BF16, rel)
+    for m in (led, led2):
+        assert ((m.mass[0].cpu().double() - p[0].sum(1)).abs() <= p[0].sum(1) * (rel + 2.0 ** -20)).all()
+    kept = torch.sort(torch.argsort(led.mass[0].cpu(), dim=-1, descending=True, stable=True)[:, :50], dim=-1).values
+    cache.evict(table, lens, n, led, 50)
+    assert torch.equal(torch.sort(led.positions[0, :, :50].cpu().long(), dim=-1).values, kept) and cache.status() == 0
+    rows = planes[0].flatten(0, 1)[table[0, t // page].long() * page + t % page].cpu()
+    for h in range(H):
+        assert torch.equal(rows[:50, h], k[led.positions[0, h, :50].cpu().long(), h])
+    assert not planes[0][:64].any()
+
+
+def test_layouts_of_small_tensors():
+    """Lengths and tables as views, a table shared by all rows, more rows of lengths than sequences."""
+    s = Setup([70, 70, 70], 2, 128, seed=31)
+    q = s.query(3, heads=8).cuda()
+    want = s.cache.decode(q, s.dtable, s.dlens, 70)
+    lens = torch.tensor([[70, 1], [70, 2], [70, 3], [5, 5]], dtype=torch.int32, device="cuda")[:, 0]
+    assert torch.equal(s.cache.decode(q, s.dtable, lens, 70), want)
+    shared = s.dtable[:1].expand(3, -1)
+    a = s.cache.decode(q, shared, s.dlens, 70)
+    assert torch.equal(a[0], want[0]) and not torch.equal(a[1], want[1])
+    window = s.query(6, 5, heads=8).cuda()[::2]
+    x, y = AttentionLedger(3, 2, 70, "cuda"), AttentionLedger(3, 2, 70, "cuda")
+    s.cache.observe(window, shared, s.dlens, 70, x)
+    s.cache.observe(window.contiguous(), shared.contiguous(), s.dlens, 70, y)
+    assert torch.equal(x.mass, y.mass) and s.cache.status() == 0
+
+
+def test_a_cache_made_and_used_on_another_stream():
+    side = torch.cuda.Stream()
+    s = Setup([500, 30], 2, 128, seed=32)
+    q = s.query(2, heads=8).cuda()
+    want = s.cache.decode(q, s.dtable, s.dlens, 500)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        cache = PagedKVCache(s.spec, s.cache.key_cache, s.cache.value_cache)
+        outs = [cache.decode(q, s.dtable, s.dlens, 500) for _ in range(5)]
+    side.synchronize()
+    assert all(torch.equal(o, want) for o in outs) and cache.status() == 0
+
+
+def test_a_long_trim_captured():
+    """A cluster of CTAs a row, replayed: the same trim each time, since the ledger it reads is left alone."""
+    s = Setup([20000, 100], 1, 64, 128, seed=33)
+    led, out = AttentionLedger(2, 1, 20000, "cuda"), AttentionLedger(2, 1, 20000, "cuda")
+    led.mass.copy_(torch.rand(led.mass.shape, generator=s.gen))
+    want = _evict_reference(s, led, s.lens, 3000, 50)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lens = s.cache.evict(s.dtable, s.dlens, 20000, led, 3000, 50, out=out)
+    for _ in range(3):
+        out.mass.fill_(3.0)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert lens.tolist() == want[4] and same_bits(out.mass, want[2]) and torch.equal(out.positions.cpu(), want[3])
+    assert same_bits(s.cache.key_cache, want[0]) and same_bits(s.cache.value_cache, want[1])
+
+
 def test_random_batches():
     """Lengths, heads, pages and types at random: decode with a ledger against 64 bits."""
     rng = random.Random(5)

@@ -113,6 +113,12 @@ class AttentionLedger:
         self.seen[at] = 0
 
 
+def _settle(device: torch.device) -> None:
+    """Wait for the current stream of `device`."""
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+
+
 class PagedKVCache:
     """One layer's exact paged cache over an engine's planes.
 
@@ -142,6 +148,8 @@ class PagedKVCache:
                                key_cache.shape[0], spec.num_kv_heads, spec.head_dim, *key_cache.stride()[:3])
         self.addr = C.addressof(self.c)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        if not torch.cuda.is_available() or not torch.cuda.is_current_stream_capturing():
+            _settle(self.device)        # the word is zero for whatever stream comes first
         self._tickets: dict = {}        # by stream
 
     @classmethod
