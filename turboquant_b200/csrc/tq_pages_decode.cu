@@ -299,10 +299,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
         rd = rd + 1 == NST ? 0 : rd + 1;
         issue();
     };
-    if (units > 0) look_up();
-#pragma unroll 1
-    for (int i = 0; i < NST; ++i) issue();
-
     // ---- the current (sequence, head)
     uint32_t qf[NT][KS][2];
     float acc[KS][NT][4], m[NT][2], l[NT][2];
@@ -408,9 +404,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
     int flag = 0;
     bool open = false;          // the last piece goes on behind this warp's share
     if (units > 0) {
+        look_up();
         flag = at.c == 0 ? 3 : (at.nch - at.c <= units ? 1 : 2);
         begin();
     }
+    // the query has been asked for: the first keys come behind it
+#pragma unroll 1
+    for (int i = 0; i < NST; ++i) issue();
+
     // ldmatrix: this lane's row and 16-byte piece of a 16 x 16 tile of the keys, and of the values (transposed)
     const uint32_t k_at = (((lane >> 3) & 1) * 8 + (lane & 7)) * ROWB + (((lane >> 4) ^ (lane & 7)) << 4);
     const uint32_t v_at = ((lane >> 4) * 8 + (lane & 7)) * ROWB + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
@@ -597,13 +598,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
                 if (tid < 2) {
                     s_last[tid] = 0;
                     if (s_event[tid].valid) {
-                        __threadfence();
                         const int from = s_event[tid].first / share, to = (s_event[tid].first + s_event[tid].nch - 1) / share;
-                        if (atomicAdd(&p.tickets[from], 1) == to - from) {
+                        int before;                       // releases this CTA's pieces, acquires the others'
+                        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + from) : "memory");
+                        if (before == to - from) {
                             p.tickets[from] = 0;          // for the next launch
                             s_last[tid] = to - from + 1;
                         }
-                        __threadfence();
                     }
                 }
             }
