@@ -113,12 +113,6 @@ class AttentionLedger:
         self.seen[at] = 0
 
 
-def _settle(device: torch.device) -> None:
-    """Wait for the current stream of `device`."""
-    if device.type == "cuda":
-        torch.cuda.current_stream(device).synchronize()
-
-
 class PagedKVCache:
     """One layer's exact paged cache over an engine's planes.
 
@@ -126,7 +120,8 @@ class PagedKVCache:
     (2, num_blocks, block_size, H, D) tensor its two halves), head_dim contiguous, rows 16-byte aligned.
 
     The calls launch on the current stream of the cache's device and synchronise nothing; each has scratch memory of its own,
-    so that calls on several streams, and captured ones, do not meet (two that touch the same pages are the caller's to order).
+    so that calls on several streams, and captured ones, do not meet (two that touch the same pages are the caller's to order,
+    and so is a stream's first call behind the making of the object, as for any tensor).
     An index that would lead outside the pages is skipped, its token taken for absent, and `status` reports it.
     """
 
@@ -148,8 +143,6 @@ class PagedKVCache:
                                key_cache.shape[0], spec.num_kv_heads, spec.head_dim, *key_cache.stride()[:3])
         self.addr = C.addressof(self.c)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        if not torch.cuda.is_available() or not torch.cuda.is_current_stream_capturing():
-            _settle(self.device)        # the word is zero for whatever stream comes first
         self._tickets: dict = {}        # by stream
 
     @classmethod
