@@ -210,3 +210,12 @@ def test_refusals_of_the_class(cache):
         with pytest.raises(ValueError):
             cache.evict(table, lens, 64, led, budget, recent)
     assert cache.status() == 0
+
+
+@pytest.mark.parametrize("batch,tokens,code", [(16, (1 << 30) - 32, SHAPE), (16, (1 << 30) - (1 << 19), 0), (15, 1 << 30, 0)])
+def test_a_list_rounded_up_to_shares_stays_in_32_bits(lib, call, batch, tokens, code):
+    """2^31 - 64 units of 16 tokens and head fit, but not once every CTA's share is rounded up."""
+    call.batch.max_seq_len, call.batch.batch = tokens, batch
+    call.batch.table_width = call.batch.table_stride = 1 << 26
+    size = C.c_size_t(0)
+    assert lib.tq_pages_decode_scratch_bytes(C.byref(call.pages), C.byref(call.batch), 8, 0, C.byref(size)) == code

@@ -96,7 +96,9 @@ inline Pages pages_of(const tq_pages* g) {
     return Pages{static_cast<uint8_t*>(g->key), static_cast<uint8_t*>(g->value), g->num_blocks, g->stride_block * 2,
                  g->stride_token * 2, g->stride_head * 2, g->block_size, g->num_kv_heads, divisor(g->block_size)};
 }
-// A batch has at most 2^31 units of 16 tokens and head, and a table row covers max_seq_len tokens.
+// What a list of work (units of a decode, tiles of an observation) may hold: its indices, rounded up to shares, stay below 2^31.
+constexpr int64_t MAX_UNITS = ((int64_t)1 << 31) - (1 << 20);
+// A table row covers max_seq_len tokens.
 inline int batch_check(const tq_pages* g, const tq_pages_batch* q) {
     if (!q || !q->block_tables || !q->seq_lens) return TQ_ERR_NULL;
     if (q->batch < 1 || q->max_seq_len < 1 || q->table_width < 1 || q->table_stride < q->table_width) return TQ_ERR_SHAPE;

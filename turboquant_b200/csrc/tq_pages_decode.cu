@@ -753,7 +753,7 @@ int decode_check(const tq_pages* g, const tq_pages_batch* q, int32_t num_q_heads
     if (rc != TQ_OK) return rc;
     if (num_q_heads < 1 || num_q_heads % g->num_kv_heads != 0) return TQ_ERR_SHAPE;
     const int64_t heads = (int64_t)g->num_kv_heads * row_tiles(num_q_heads / g->num_kv_heads);
-    if (heads * q->batch * (((int64_t)q->max_seq_len + 15) / 16) >= ((int64_t)1 << 31)) return TQ_ERR_SHAPE;
+    if (heads * q->batch * (((int64_t)q->max_seq_len + 15) / 16) > MAX_UNITS) return TQ_ERR_SHAPE;
     return TQ_OK;
 }
 

@@ -440,7 +440,7 @@ int observe_check(const tq_pages* g, const tq_pages_batch* q, int window, int Qh
     if (window < 1 || Qh < 1 || Qh % g->num_kv_heads != 0) return TQ_ERR_SHAPE;
     if ((int64_t)window * (Qh / g->num_kv_heads) > (1 << 20)) return TQ_ERR_SHAPE;
     const int64_t lists = (int64_t)q->batch * g->num_kv_heads * row_tiles_of(g, window, Qh);
-    if (lists * (((int64_t)q->max_seq_len + OB_TILE - 1) / OB_TILE) >= ((int64_t)1 << 31)) return TQ_ERR_SHAPE;
+    if (lists * (((int64_t)q->max_seq_len + OB_TILE - 1) / OB_TILE) > MAX_UNITS) return TQ_ERR_SHAPE;
     return TQ_OK;
 }
 template <int D>
