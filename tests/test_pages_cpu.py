@@ -82,8 +82,8 @@ def test_calls_are_checked(lib, call):
     short = _lib.tq_pages_ledger(base, base, base, base, 63)
     missing = _lib.tq_pages_ledger(base, None, base, base, 64)
     assert evict(led=short) == RANGE and evict(led=missing) == NULL
-    assert lib.tq_pages_evict_scratch_bytes(C.byref(c.pages), C.byref(c.batch), 8, C.byref(size)) == 0 and size.value == 6 * 4 + 6 * 8 * 8
-    assert lib.tq_pages_evict_scratch_bytes(C.byref(c.pages), C.byref(c.batch), 60, C.byref(size)) == 0 and size.value == 6 * 4 + 6 * 4 * 8
+    assert lib.tq_pages_evict_scratch_bytes(C.byref(c.pages), C.byref(c.batch), 8, C.byref(size)) == 0 and size.value == 6 * 4 + 6 * 8 * 16
+    assert lib.tq_pages_evict_scratch_bytes(C.byref(c.pages), C.byref(c.batch), 60, C.byref(size)) == 0 and size.value == 6 * 4 + 6 * 4 * 16
     assert lib.tq_pages_evict_scratch_bytes(C.byref(c.pages), C.byref(c.batch), 100, C.byref(size)) == 0 and size.value == 6 * 4
 
 

@@ -64,9 +64,14 @@ __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteP
 // are left between the ends, one warp settles those alone.  Lane-striped slots (warp * 32 * KPT + i * 32 + lane) let a ballot
 // count a row and keep every list in ascending order.
 //
-// Bound by the chain of loads, exchanges and lists: 6 us for 300 slots, 10 for 512 rows of 2112 (four CTAs an SM at 56 registers; at
-// 40 they spill and it is 16 longer), 20 for 32 rows of up to 32768 in clusters of four (a cluster's exchange takes 1.6 us, a CTA's
-// 0.2: candidates go to one CTA as soon as it holds them).
+// A token that moves goes into a list with its mass and position; the second launch, which needs the list for the rows, puts them in
+// their places (in this one a mover would have to wait for the holes of the other CTAs: 512 rows of 2112 21.0 us in the place of
+// 19.9, 32 of up to 32768 46.6 in the place of 45.0, one of 32768 28 in the place of 25).
+//
+// Bound by the chain of loads, exchanges and lists.  Both launches take 9.7 us for 300 slots, 19.9 for 512 rows of 2112, of which
+// moving the rows is 8 (four CTAs an SM at 56 registers; at 40 they spill and it is 16 longer), 45.0 for 32 rows of up to 32768 in
+// clusters of four, of which moving is 20 (a cluster's exchange takes 1.6 us, a CTA's 0.2: candidates go to one CTA as soon as it
+// holds them).
 struct EvictParams {
     Pages g;
     Batch q;
@@ -80,6 +85,8 @@ struct EvictParams {
     int budget, recent;
     int32_t* dst;                  // [batch * H][list]
     int32_t* src;
+    float* src_mass;               // of the tokens that move
+    int32_t* src_positions;
     int32_t* count;                // [batch * H]
     int list;
     int32_t* status;
@@ -189,7 +196,9 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
     const int32_t* positions = p.positions + row * p.stride;
     float* out_mass = p.out_mass + row * p.out_stride;
     int32_t* out_positions = p.out_positions + row * p.out_stride;
-    int32_t *dst = p.dst + (int64_t)row * p.list, *src = p.src + (int64_t)row * p.list;
+    const int64_t first = (int64_t)row * p.list;
+    int32_t *dst = p.dst + first, *src = p.src + first, *src_positions = p.src_positions + first;
+    float* src_mass = p.src_mass + first;
     const int span = ctas * warps * 32 * KPT, rounds = LONG ? (n + span - 1) / span : 1;
 
     uint32_t key[KPT];                 // 0: not in the cache
@@ -403,7 +412,6 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
             my_movers += __popc(__ballot_sync(0xffffffffu, t >= m && stays));
             kept |= (uint32_t)stays << i;
         }
-        // all loads in front of the first store: the arrays may be the same ones
         float x[KPT];
         int pos[KPT];
 #pragma unroll
@@ -427,23 +435,16 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
                 hole_at += __popc(hole);
             }
             if (t < m && stays) out_mass[t] = x[i], out_positions[t] = pos[i];
+            if (trims) {
+                const uint32_t mover = __ballot_sync(0xffffffffu, t >= m && stays);
+                const int at = mover_at + __popc(mover & below);
+                if (t >= m && stays) src[at] = t, src_mass[at] = x[i], src_positions[at] = pos[i];
+                mover_at += __popc(mover);
+            }
         }
-        if (!trims) continue;
-        team.sync();                                       // every hole that a mover of this round takes has been noted: holes lie before movers
-        int at[KPT], to[KPT];
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const bool moves = t0 + i * 32 >= m && ((kept >> i) & 1);
-            const uint32_t mover = __ballot_sync(0xffffffffu, moves);
-            at[i] = moves ? mover_at + __popc(mover & below) : -1;
-            mover_at += __popc(mover);
-            if (moves) to[i] = __ldcg(dst + at[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < KPT; ++i)
-            if (at[i] >= 0) src[at[i]] = t0 + i * 32, out_mass[to[i]] = x[i], out_positions[to[i]] = pos[i];
     }
-    team.sync();                                           // in place: nothing is cleared before it has been read
+    // in place: nothing is cleared before it has been read (in a row that the team holds, before the last exchange)
+    if (LONG) team.sync();
     for (int64_t t = m + rank * (int)blockDim.x + (int)threadIdx.x; t < p.out_stride; t += ctas * blockDim.x) {
         out_mass[t] = 0.f;
         out_positions[t] = -1;
@@ -452,7 +453,7 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
 }
 
 // The moves of all (sequence, kv head) rows: a group of D/8 lanes copies a key row and a value row.  Bound by HBM: 3500 rows of each of
-// 32 heads of 128, 115 MB: 20 us.
+// 32 heads of 128, 115 MB: 20 us (two rows a group at a time 21.5, four 25: more groups beat more loads of one).
 template <int D>
 __global__ void __launch_bounds__(256) tq_pages_move_kernel(const EvictParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -468,7 +469,12 @@ __global__ void __launch_bounds__(256) tq_pages_move_kernel(const EvictParams p)
     const int count = p.count[row];
     const int32_t* table = p.q.table + (int64_t)b * p.q.table_stride;
     for (int j = blockIdx.y * PER + threadIdx.x / LPR; j < count; j += gridDim.y * PER) {
-        const int from = p.src[(int64_t)row * p.list + j], to = p.dst[(int64_t)row * p.list + j];
+        const int64_t at = (int64_t)row * p.list + j;
+        const int from = p.src[at], to = p.dst[at];
+        if (threadIdx.x % LPR == 0) {
+            p.out_mass[row * p.out_stride + to] = p.src_mass[at];
+            p.out_positions[row * p.out_stride + to] = p.src_positions[at];
+        }
         const int eb = table[from / p.g.page], tb = table[to / p.g.page];
         if ((uint32_t)eb >= (uint64_t)p.g.num_blocks || (uint32_t)tb >= (uint64_t)p.g.num_blocks) {
             atomicCAS(p.status, 0, (int)TQ_ERR_RANGE);
@@ -524,7 +530,7 @@ extern "C" int tq_pages_evict_scratch_bytes(const tq_pages* pages, const tq_page
     const int rc = evict_check(pages, batch, budget);
     if (rc != TQ_OK) return rc;
     const size_t rows = (size_t)batch->batch * pages->num_kv_heads;
-    *out = rows * 4 + rows * evict_list(batch, budget) * 8;
+    *out = rows * 4 + rows * evict_list(batch, budget) * 16;
     return TQ_OK;
 }
 
@@ -563,6 +569,8 @@ extern "C" int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch
     p.count = static_cast<int32_t*>(scratch);
     p.dst = p.count + rows;
     p.src = p.dst + rows * p.list;
+    p.src_positions = p.src + rows * p.list;
+    p.src_mass = reinterpret_cast<float*>(p.src_positions + rows * p.list);
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     tq_note_launch(st, TQ_LAUNCH_WAITED);      // writes rows that a store may read next
