@@ -68,8 +68,8 @@ __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteP
 // their places (in this one a mover would have to wait for the holes of the other CTAs: 512 rows of 2112 21.0 us in the place of
 // 19.9, 32 of up to 32768 46.6 in the place of 45.0, one of 32768 28 in the place of 25).
 //
-// Bound by the chain of loads, exchanges and lists.  Both launches take 9.7 us for 300 slots, 19.9 for 512 rows of 2112, of which
-// moving the rows is 8 (four CTAs an SM at 56 registers; at 40 they spill and it is 16 longer), 45.0 for 32 rows of up to 32768 in
+// Bound by the chain of loads, exchanges and lists.  Both launches take 9.6 us for 300 slots, 19.3 for 512 rows of 2112, of which
+// moving the rows is 8 (four CTAs an SM at 56 registers; at 40 they spill and it is 16 longer), 43.5 for 32 rows of up to 32768 in
 // clusters of four, of which moving is 20 (a cluster's exchange takes 1.6 us, a CTA's 0.2: candidates go to one CTA as soon as it
 // holds them).
 struct EvictParams {
@@ -453,38 +453,45 @@ __global__ void __maxnreg__(56) tq_pages_evict_kernel(const EvictParams p) {
 }
 
 // The moves of all (sequence, kv head) rows: a group of D/8 lanes copies a key row and a value row.  Bound by HBM: 3500 rows of each of
-// 32 heads of 128, 115 MB: 20 us (two rows a group at a time 21.5, four 25: more groups beat more loads of one).
+// 32 heads of 128, 115 MB: 20 us (two rows a group at a time 21.5, four 25: more groups beat more loads of one).  The list is read
+// beside its length: 0.6 us of a call's chain.
 template <int D>
 __global__ void __launch_bounds__(256) tq_pages_move_kernel(const EvictParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int LPR = D / 8, PER = 256 / LPR;
     const int row = blockIdx.x, b = row / p.g.H, h = row % p.g.H;
+    const int32_t* table = p.q.table + (int64_t)b * p.q.table_stride;
+    const int64_t first = (int64_t)row * p.list, o = (threadIdx.x % LPR) * 16 + h * p.g.sh;
+    const bool leads = threadIdx.x % LPR == 0;             // of the group: the ledger's entry is its
+    int j = blockIdx.y * PER + threadIdx.x / LPR, from, to, position;
+    float mass;
+    auto look_up = [&]() {
+        from = p.src[first + j], to = p.dst[first + j];
+        if (leads) mass = p.src_mass[first + j], position = p.src_positions[first + j];
+    };
+    if (j < p.list) look_up();                             // beside the count, which says whether it is one
+    const int count = p.count[row];
+    while (j < count) {
+        const int fp = p.g.by_page.quotient(from), tp = p.g.by_page.quotient(to), eb = table[fp], tb = table[tp];
+        if (leads) p.out_mass[row * p.out_stride + to] = mass, p.out_positions[row * p.out_stride + to] = position;
+        if ((uint32_t)eb < (uint64_t)p.g.num_blocks && (uint32_t)tb < (uint64_t)p.g.num_blocks) {
+            const int64_t s = eb * p.g.sb + (int64_t)(from - fp * p.g.page) * p.g.st + o;
+            const int64_t d = tb * p.g.sb + (int64_t)(to - tp * p.g.page) * p.g.st + o;
+            const uint4 k = *reinterpret_cast<const uint4*>(p.g.k + s), v = *reinterpret_cast<const uint4*>(p.g.v + s);
+            *reinterpret_cast<uint4*>(p.g.k + d) = k;
+            *reinterpret_cast<uint4*>(p.g.v + d) = v;
+        } else {
+            atomicCAS(p.status, 0, (int)TQ_ERR_RANGE);
+        }
+        j += gridDim.y * PER;
+        if (j < count) look_up();
+    }
     if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) {   // here, not in the first launch: other heads of the sequence read them there
         const int n = seq_len(p.q, b, p.status), held = p.held[b], seen = p.seen[b];
         p.new_lens[b] = min(n, p.budget);
         p.out_seen[b] = seen + n - held;
         p.out_held[b] = min(n, p.budget);
-    }
-    const int count = p.count[row];
-    const int32_t* table = p.q.table + (int64_t)b * p.q.table_stride;
-    for (int j = blockIdx.y * PER + threadIdx.x / LPR; j < count; j += gridDim.y * PER) {
-        const int64_t at = (int64_t)row * p.list + j;
-        const int from = p.src[at], to = p.dst[at];
-        if (threadIdx.x % LPR == 0) {
-            p.out_mass[row * p.out_stride + to] = p.src_mass[at];
-            p.out_positions[row * p.out_stride + to] = p.src_positions[at];
-        }
-        const int eb = table[from / p.g.page], tb = table[to / p.g.page];
-        if ((uint32_t)eb >= (uint64_t)p.g.num_blocks || (uint32_t)tb >= (uint64_t)p.g.num_blocks) {
-            atomicCAS(p.status, 0, (int)TQ_ERR_RANGE);
-            continue;
-        }
-        const int64_t o = (threadIdx.x % LPR) * 16 + h * p.g.sh;
-        const int64_t s = eb * p.g.sb + (from % p.g.page) * p.g.st + o, d = tb * p.g.sb + (to % p.g.page) * p.g.st + o;
-        const uint4 k = *reinterpret_cast<const uint4*>(p.g.k + s), v = *reinterpret_cast<const uint4*>(p.g.v + s);
-        *reinterpret_cast<uint4*>(p.g.k + d) = k;
-        *reinterpret_cast<uint4*>(p.g.v + d) = v;
     }
 }
 
