@@ -1,0 +1,66 @@
+"""The exact paged cache on the GPU where its numbers, lengths and layouts come to their ends, against 64-bit torch."""
+
+import math
+
+import pytest
+import torch
+
+from tests import pages_oracle as O
+from turboquant_b200 import AttentionLedger, ExactCacheSpec, PagedKVCache
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+RANGE = -7
+
+
+def cache_over(k, v, page, seed=0):
+    """A cache that holds k / v (batch, n, H, D) in pages in random order -> cache, table, lengths (all n)."""
+    b, n, h, d = k.shape
+    width = -(-n // page)
+    cache = PagedKVCache.allocate(ExactCacheSpec(d, h, block_size=page, dtype=k.dtype), b * width, "cuda")
+    table = torch.randperm(b * width, generator=torch.Generator().manual_seed(seed)).int().view(b, width)
+    for plane, x in ((cache.key_cache, k), (cache.value_cache, v)):
+        padded = torch.zeros(b, width * page, h, d, dtype=k.dtype)
+        padded[:, :n] = x
+        plane[table.flatten().long().cuda()] = padded.view(b * width, page, h, d).cuda()
+    return cache, table.cuda(), torch.full((b,), n, dtype=torch.int32, device="cuda")
+
+
+def score_error(q, k, scale):
+    """Relative error of a softmax weight: a score is a sum of exact products held in 32 bits, at most D / 16 <= 16 additions that
+    lose 2^-22 of the largest partial sum each, once in the score and once in the reference of the normalisation; exponentials
+    and sums lose some 2^-20."""
+    size = (q.abs().amax() * k.abs().sum(-1).amax()).item() * scale
+    return 2 * 16 * 2.0 ** -22 * size + 2.0 ** -19
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("D,H,G,b,n", [(128, 4, 4, 300, 200), (64, 2, 16, 280, 330), (256, 2, 1, 200, 250), (128, 1, 2, 1, 20011)])
+def test_small_weights_under_a_large_one_with_no_value(D, H, G, b, n, dtype):
+    """The first token of sequence b lies b % 28 octaves above the others and has a value of zeros: what is left of the output are
+    the small weights."""
+    g = torch.Generator().manual_seed(D + n)
+    q, k = torch.zeros(b, H * G, D), torch.zeros(b, n, H, D)
+    q[..., 1:], k[..., 1:] = 0.5 * torch.randn(b, H * G, D - 1, generator=g), 0.3 * torch.randn(b, n, H, D - 1, generator=g)
+    q[..., 0] = 8.0
+    octaves = torch.arange(b) % 28 if b > 1 else torch.tensor([24])
+    k[:, 0, :, 0] = (octaves * math.log(2.0) * math.sqrt(D) / 8.0)[:, None]
+    v = 0.5 + torch.randn(b, n, H, D, generator=g)
+    v[:, 0] = 0.0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    cache, table, lens = cache_over(k, v, 16)
+    led = AttentionLedger(b, H, n, "cuda")
+    out = cache.decode(q.cuda(), table, lens, n).cpu().double().view(b, H, G, D)
+    assert torch.equal(cache.decode(q.cuda(), table, lens, n, ledger=led).cpu().double().view(b, H, G, D), out)
+    p = torch.softmax(torch.einsum("bhgd,bnhd->bhgn", q.double().view(b, H, G, D), k.double()) / math.sqrt(D), -1)
+    ref, size = torch.einsum("bhgn,bnhd->bhgd", p, v.double()), torch.einsum("bhgn,bnhd->bhgd", p, v.double().abs())
+    rel = score_error(q.double(), k.double(), D ** -0.5)
+    # The output's rounding is half a step; a weight of two 16-bit numbers is off by 2^-18 (bf16) or 2^-22 (fp16) of itself, or
+    # where fp16 ends, 2^-15 2^-25 = 2^-40 of the largest weight, which is at most 1; sums of 32 bits, at most n / 16 times two
+    # additions in a chain that lose 2^-22 of the magnitudes each.
+    lost = size * (rel + 2.0 ** -18 + n / 8 * 2.0 ** -22) + (2.0 ** -40 if dtype is FP16 else 0.0) * v.double().abs().sum(1).view(b, H, 1, D)
+    half = ref.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -6) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    over = ((out - ref).abs() - lost - half).amax((1, 2, 3))
+    assert (over <= 0).all(), (over.max().item(), octaves[over > 0].unique().tolist())
+    added = p.sum(2)
+    assert ((led.mass.cpu().double() - added).abs() <= added * (rel + (G + 1) * 2.0 ** -24)).all() and cache.status() == 0

@@ -20,8 +20,12 @@
 //
 // Products: S^T = K Q^T and O^T = V^T P^T as m16n8k16, tokens resp. channels in the 16 rows, eight query heads in the columns,
 // so that a group of up to eight pads nothing else.  tcgen05 would want 128 rows of operands through shared memory for eight
-// useful columns; the tensor pipe is not what bounds this.  P goes into the second product as two 16-bit numbers (value and
-// rest, 2^-16 relative): one alone would cost as much precision as the rounding of the output.
+// useful columns; the tensor pipe is not what bounds this.  P goes into the second product as two 16-bit numbers, value and
+// rest: one alone would cost as much precision as the rounding of the output.  Two bf16 numbers leave 2^-18 of a weight.  Two
+// fp16 numbers leave 2^-22 of it, but nothing below half of fp16's smallest step, 2^-25, while a value row of zeros under the
+// largest weight (a sink) makes the small weights all of the output: so fp16 weights are multiplied by 2^15 before they are
+// split, and the factor is taken off again with the division by the sum.  What is lost of a weight is then at most 2^-40 of the largest
+// one of the warp's share: up to 32768 values of size one, no more than half of the smallest step of an fp16 output.
 #include "tq_pages.cuh"
 
 using namespace tqpg;
@@ -98,6 +102,9 @@ __device__ __forceinline__ float2 unpack(uint32_t w) {
     if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+// The factor on the weights that go into the second product, and so on its sums (the sums of the weights are without it).
+template <bool BF16>
+constexpr float LIFT = BF16 ? 1.f : 32768.f;
 // 2^(m - ref) where both may be -inf (nothing seen yet)
 __device__ __forceinline__ float weight(float m, float ref) { return m == -INFINITY ? 0.f : ex2(m - ref); }
 
@@ -342,7 +349,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
         const int64_t row0 = first_row(b, h, rt);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float i0 = l[nt][0] == 0.f ? 0.f : 1.f / l[nt][0], i1 = l[nt][1] == 0.f ? 0.f : 1.f / l[nt][1];
+            const float i0 = l[nt][0] == 0.f ? 0.f : 1.f / LIFT<BF16> / l[nt][0], i1 = l[nt][1] == 0.f ? 0.f : 1.f / LIFT<BF16> / l[nt][1];
             uint8_t* o = p.out + (row0 + nt * 8 + g) * ROWB + t4 * 4;
 #pragma unroll
             for (int ct = 0; ct < KS; ++ct) {
@@ -488,9 +495,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
             const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float a = ex2(s[nt][2 * k] - r0), c = ex2(s[nt][2 * k + 1] - r1);
+                float a = ex2(s[nt][2 * k] - r0), c = ex2(s[nt][2 * k + 1] - r1);
                 l[nt][0] += a;
                 l[nt][1] += c;
+                a *= LIFT<BF16>;
+                c *= LIFT<BF16>;
                 const uint32_t h = pack<BF16>(a, c);
                 const float2 back = unpack<BF16>(h);
                 hi[nt][k] = transpose8(h);
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) tq_pages_decode_kern
             }
             using E = TqElem<BF16 ? TQ_BF16 : TQ_F16>;
             const int64_t o = (row0 + row) * D + ct * 16 + gg;
-            const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+            const float i0 = l0 == 0.f ? 0.f : 1.f / LIFT<BF16> / l0, i1 = l1 == 0.f ? 0.f : 1.f / LIFT<BF16> / l1;
             E::store(p.out, o, a.x * i0);
             E::store(p.out, o + 8, a.z * i0);
             if (row + 1 < rows) {
