@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import pages_oracle as O
-from turboquant_b200 import AttentionLedger, ExactCacheSpec, PagedKVCache
+from turboquant_b200 import AttentionLedger, CompressedCacheSpec, CompressedPagedKVCache, ExactCacheSpec, PagedKVCache
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -64,3 +64,29 @@ def test_small_weights_under_a_large_one_with_no_value(D, H, G, b, n, dtype):
     assert (over <= 0).all(), (over.max().item(), octaves[over > 0].unique().tolist())
     added = p.sum(2)
     assert ((led.mass.cpu().double() - added).abs() <= added * (rel + (G + 1) * 2.0 ** -24)).all() and cache.status() == 0
+
+
+@pytest.mark.parametrize("which", ["returned", "held"])
+def test_lengths_of_an_eviction_go_straight_into_the_compressed_cache(which):
+    """The lengths that an eviction writes, read by the launch behind it: the same bits as with lengths that lay there before."""
+    b, h, n = 40, 2, 600
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(b, n, h, 128, generator=g).to(BF16) for _ in range(2))
+    exact, table, lens = cache_over(k, v, 16)
+    packed = CompressedPagedKVCache.allocate(CompressedCacheSpec(128, h, 3, 2), b * 40, "cuda")
+    slots = torch.cat([torch.arange(n) + 640 * i for i in range(b)]).cuda()
+    packed.write(k.view(-1, h, 128).cuda(), v.view(-1, h, 128).cuda(), slots)
+    tables = torch.arange(b * 40, dtype=torch.int32, device="cuda").view(b, 40)
+    q = torch.randn(b, 4 * h, 128, generator=g).to(BF16).cuda()
+    led = AttentionLedger(b, h, n, "cuda")
+    wants = {}
+    for budget in (500, 17, 333):
+        wants[budget] = packed.decode(q, tables, torch.full((b,), budget, dtype=torch.int32, device="cuda"), n).clone()
+    assert not torch.equal(wants[500], wants[17])
+    for i in range(30):
+        budget = (500, 17, 333)[i % 3]
+        led.reset()
+        torch.full((b,), 10 ** 6 + i, dtype=torch.int32, device="cuda")       # what the new lengths' memory held before
+        new = exact.evict(table, lens, n, led, budget)
+        got = packed.decode(q, tables, new if which == "returned" else led.held, n)
+        assert torch.equal(got, wants[budget]) and packed.workspace.status() == 0

@@ -352,7 +352,7 @@ int launch_qprep(const void* q, int dt, int64_t nvec, int D, const float* pi_t, 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its matrix loads may run under the previous kernel's tail
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;   // behind a store too: the pool is not touched here
+    cfg.numAttrs = tq_prep_may_overlap(tq_last_launch(st)) ? 1 : 0;   // behind a store too: the pool is not touched here
     tq_note_prep_launch(st);
     cfg.stream = st;
     cfg.blockDim = dim3(256);
@@ -1113,7 +1113,7 @@ extern "C" int tq_decode_host_io(const tq_consts* consts, const tq_pool* pool, c
             attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
             attr[0].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr;
-            cfg.numAttrs = 1;
+            cfg.numAttrs = tq_prep_may_overlap(tq_last_launch(st)) ? 1 : 0;
             tq_note_prep_launch(st);
             if (cudaLaunchKernelEx(&cfg, tq_stage_in_kernel, (const uint4*)host_in, (uint4*)dev_in, (int)(in_bytes / 16)) !=
                 cudaSuccess)

@@ -580,7 +580,7 @@ extern "C" int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch
     p.src_mass = reinterpret_cast<float*>(p.src_positions + rows * p.list);
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
-    tq_note_launch(st, TQ_LAUNCH_WAITED);      // writes rows that a store may read next
+    tq_note_launch(st, TQ_LAUNCH_LENGTHS);     // writes rows that a store may read next, and lengths that a decode may
     // as many CTAs a row as it takes to hold its keys in registers, up to eight; no more warps than hold them
     const int n = batch->max_seq_len, cta = EV_WARPS * 32 * EV_KPT;
     const int ctas = n <= cta ? 1 : n <= 2 * cta ? 2 : n <= 4 * cta ? 4 : EV_CTAS;

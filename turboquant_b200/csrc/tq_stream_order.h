@@ -13,6 +13,9 @@
 //     A decode kernel directly behind a store is launched in plain stream order.  The fp32 store and the planes' converter let
 //     nobody begin, but a launch that begins when they have finished has not waited for them either, and only the wait makes
 //     what they wrote visible: the same holds behind them.
+//   * an eviction writes lengths (the new ones, and a ledger's `held`), which the decode family reads at its entry, records waited
+//     for or not.  Behind one, a kernel that lets its dependents begin at entry is launched in plain stream order, as is a
+//     decode kernel; launches that wait before they let anyone begin need nothing.
 // Kernels of other libraries between two of ours never start early and only make the order stricter.  Of a stream that has no
 // note - the library has not seen it, or other streams' notes took its place - anything may be in flight.
 #pragma once
@@ -27,15 +30,18 @@ enum TqLaunchKind {
     TQ_LAUNCH_PREP_BEHIND_STORE = 4,   // prepares a call, a store may still be in flight
     TQ_LAUNCH_WAITED = 5,              // writes no pool (rows perhaps), and waits before it lets anyone begin
     TQ_LAUNCH_STORE_PLAIN = 6,         // writes the pool, in plain stream order, and lets nobody begin before it has finished
+    TQ_LAUNCH_LENGTHS = 7,             // writes rows and lengths, and waits before it lets anyone begin
 };
 
 // what a launch is noted as that prepares a call (and neither reads nor writes the pool) and lets its dependents begin at once
 inline int tq_kind_of_prep(int ahead) {
     return ahead == TQ_LAUNCH_DECODE || ahead == TQ_LAUNCH_NEUTRAL || ahead == TQ_LAUNCH_WAITED ? TQ_LAUNCH_DECODE : TQ_LAUNCH_PREP_BEHIND_STORE;
 }
-// whether a kernel that reads the pool early may be launched as a programmatic dependent (else: plain stream order) ...
+// whether it may be launched as a programmatic dependent (else: plain stream order), with readers of lengths behind it
+inline bool tq_prep_may_overlap(int ahead) { return ahead != TQ_LAUNCH_LENGTHS && ahead != TQ_LAUNCH_UNKNOWN; }
+// whether a kernel that reads the pool and lengths early may be launched as a programmatic dependent (else: plain stream order) ...
 inline bool tq_reader_may_overlap(int ahead) {
-    return ahead != TQ_LAUNCH_STORE_EARLY && ahead != TQ_LAUNCH_STORE_PLAIN && ahead != TQ_LAUNCH_UNKNOWN;
+    return ahead != TQ_LAUNCH_STORE_EARLY && ahead != TQ_LAUNCH_STORE_PLAIN && ahead != TQ_LAUNCH_LENGTHS && ahead != TQ_LAUNCH_UNKNOWN;
 }
 // ... and whether it then has to wait before its first record
 inline bool tq_pool_is_late(int ahead) { return ahead == TQ_LAUNCH_PREP_BEHIND_STORE || !tq_reader_may_overlap(ahead); }
