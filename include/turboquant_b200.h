@@ -499,6 +499,8 @@ typedef struct tq_pages_batch {
     const int32_t* seq_lens;       /* (batch), device */
     int32_t batch;
     int32_t max_seq_len;           /* host upper bound; table_width * block_size covers it */
+    const int32_t* held;           /* a ledger's, device, or NULL: nothing has been evicted.  For tq_pages_observe alone */
+    const int32_t* seen;           /* with held */
 } tq_pages_batch;
 
 /* What the tokens of `batch` cached sequences have received, kv head by kv head; rows of `max_tokens`.  Slots below held[b] have
@@ -533,7 +535,9 @@ int tq_pages_decode(const tq_pages* pages, const tq_pages_batch* batch, const vo
 
 /* The weights of the last `window` queries of every sequence alone: query (batch, window, num_q_heads, head_dim) contiguous, query
  * i of a sequence of n tokens at position n - window + i, where it sees the tokens up to its own (one before the first token
- * sees nothing); their softmax weights, summed over the window and the kv head's query heads, are added to `mass`. */
+ * sees nothing); their softmax weights, summed over the window and the kv head's query heads, are added to `mass`.  That is by
+ * slot: in a sequence that tokens have been evicted from (held[b] != seen[b]) a query among the held[b] slots, which are in no
+ * order, sees nothing and is reported. */
 int tq_pages_observe_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t window, int32_t num_q_heads, size_t* out);
 int tq_pages_observe(const tq_pages* pages, const tq_pages_batch* batch, const void* query, int32_t window, int32_t num_q_heads,
                      float scale, float* mass, int64_t mass_stride, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);

@@ -90,3 +90,55 @@ def test_lengths_of_an_eviction_go_straight_into_the_compressed_cache(which):
         new = exact.evict(table, lens, n, led, budget)
         got = packed.decode(q, tables, new if which == "returned" else led.held, n)
         assert torch.equal(got, wants[budget]) and packed.workspace.status() == 0
+
+
+def test_observing_after_an_eviction():
+    """A second prompt of a chat: windows of the tokens that came after the eviction see all that is held and each other up to their
+    own; queries further back give nothing and are reported.  A sequence that nothing was evicted from stays as it was."""
+    H, G, D, W = 2, 4, 128, 12
+    n = torch.tensor([400, 90, 300, 64])
+    g = torch.Generator().manual_seed(8)
+    k, v = torch.randn(4, 400, H, D, generator=g).to(BF16), torch.randn(4, 400, H, D, generator=g).to(BF16)
+    cache, table, _ = cache_over(k, v, 16)
+    led = AttentionLedger(4, H, 400, "cuda")
+    led.mass.copy_(torch.rand(4, H, 400, generator=g))
+    lens = cache.evict(table, n.int().cuda(), 400, led, 100, 10)      # 100 of 400, 90 as they are, 100 of 300, 64 as they are
+    assert lens.tolist() == [100, 90, 100, 64]
+    for more, early in (([12, 0, 40, 3], False), ([5, 1, 0, 12], True)):
+        now = lens + torch.tensor(more, dtype=torch.int32, device="cuda")      # slots behind hold rows already
+        led.mass.zero_()
+        q = torch.randn(4, W, H * G, D, generator=g).to(BF16)
+        cache.observe(q.cuda(), table, now, 400, led)
+        assert cache.status() == (RANGE if early else 0)
+        for b, m in enumerate(now.tolist()):
+            rows = [O.gather(plane.cpu(), table[b].cpu(), m, 16) for plane in (cache.key_cache, cache.value_cache)]
+            last = torch.arange(m - W, m)
+            if b % 2 == 0:
+                last = torch.where(last < 100, -1, last)
+            qb = q[b].double().view(W, H, G, D)
+            _, p = O.attention(qb, *rows, last=last)
+            add, rel = p.sum((0, 2)), score_error(qb, rows[0], D ** -0.5)
+            got = led.mass[b].cpu().double()
+            assert ((got[:, :m] - add).abs() <= add * (rel + (W * G + 2) * 2.0 ** -24)).all() and not got[:, m:].any()
+            assert abs(got.sum().item() - H * G * (last >= 0).sum().item()) <= 1e-3 * W * H * G
+
+
+def test_observing_after_an_eviction_with_many_rows():
+    """Windows of several row tiles, of which the first lie wholly in the part that is in no order."""
+    H, G, D, W, n = 1, 8, 64, 70, 513
+    g = torch.Generator().manual_seed(9)
+    k, v = torch.randn(1, n, H, D, generator=g).to(FP16), torch.randn(1, n, H, D, generator=g).to(FP16)
+    cache, table, lens = cache_over(k, v, 32)
+    for held, seen in ((480, 481), (500, 2000), (513, 600), (600, 700), (480, 480), (0, 0)):
+        led = AttentionLedger(1, H, n, "cuda")
+        led.held.fill_(held), led.seen.fill_(seen)
+        q = torch.randn(1, W, H * G, D, generator=g).to(FP16)
+        cache.observe(q.cuda(), table, lens, n, led)
+        evicted = seen != held
+        assert cache.status() == (RANGE if evicted and held > n - W else 0)
+        last = torch.arange(n - W, n)
+        if evicted:
+            last = torch.where(last < held, -1, last)
+        _, p = O.attention(q[0].double().view(W, H, G, D), k[0].double(), v[0].double(), last=last)
+        add, rel = p.sum((0, 2)), score_error(q.double(), k.double(), D ** -0.5)
+        assert ((led.mass[0].cpu().double() - add).abs() <= add * (rel + (W * G + W * G // 128 + 2) * 2.0 ** -24)).all()

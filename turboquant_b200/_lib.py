@@ -71,7 +71,7 @@ class tq_pages(C.Structure):
 
 class tq_pages_batch(C.Structure):
     _fields_ = [("block_tables", C.c_void_p), ("table_stride", C.c_int32), ("table_width", C.c_int32), ("seq_lens", C.c_void_p),
-                ("batch", C.c_int32), ("max_seq_len", C.c_int32)]
+                ("batch", C.c_int32), ("max_seq_len", C.c_int32), ("held", C.c_void_p), ("seen", C.c_void_p)]
 
 
 class tq_pages_ledger(C.Structure):

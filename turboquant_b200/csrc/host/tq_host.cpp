@@ -634,34 +634,6 @@ PyObject* pages_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
-// pages_observe(pages, status, query (b, window, Qh, D), tables, lens, max_len, scale | None, mass) -> status code or None
-PyObject* pages_observe(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-    HANDLE_TH_ERRORS
-    ARGS(8);
-    const at::Tensor *q = tensor_or_null(args[2]), *mass = tensor_or_null(args[7]);
-    PagesCall c;
-    if (!q || q->dim() != 4 || !pages_call(c, args[0], args[1], args[3], args[4], args[5], q->size(0))) {
-        if (PyErr_Occurred()) return nullptr;
-        Py_RETURN_NONE;
-    }
-    const int64_t d = c.pages->head_dim, qh = q->size(2), window = q->size(1);
-    const double scale = args[6] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(args[6]);
-    if (PyErr_Occurred()) return nullptr;
-    if (!on(*q, *c.status) || !q->is_contiguous() || q->size(3) != d || qh < 1 || qh > INT32_MAX || window < 1 || window > INT32_MAX ||
-        dtype_code(q->scalar_type()) != (int)c.pages->dtype || !plane_ok(mass, c, at::kFloat))
-        Py_RETURN_NONE;
-    const c10::cuda::CUDAGuard guard(c.status->get_device());
-    size_t need = 0;
-    int rc = tq_pages_observe_scratch_bytes(c.pages, &c.batch, (int32_t)window, (int32_t)qh, &need);
-    if (rc != TQ_OK) return PyLong_FromLong(rc);
-    const at::Tensor scratch = bytes_like(*q, need);
-    rc = tq_pages_observe(c.pages, &c.batch, q->data_ptr(), (int32_t)window, (int32_t)qh, (float)scale, mass->data_ptr<float>(), mass->size(2),
-                          scratch.data_ptr(), need, c.status->data_ptr<int32_t>(), stream_of(*q));
-    if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
-    return PyLong_FromLong(rc);
-    END_HANDLE_TH_ERRORS
-}
-
 // mass, positions, held, seen
 bool ledger_of(tq_pages_ledger& l, const PagesCall& c, PyObject* const* args) {
     const at::Tensor *mass = tensor_or_null(args[0]), *pos = tensor_or_null(args[1]), *held = tensor_or_null(args[2]), *seen = tensor_or_null(args[3]);
@@ -674,6 +646,38 @@ bool ledger_of(tq_pages_ledger& l, const PagesCall& c, PyObject* const* args) {
     l.seen = seen->data_ptr<int32_t>();
     l.max_tokens = (int32_t)mass->size(2);
     return true;
+}
+
+// pages_observe(pages, status, query (b, window, Qh, D), tables, lens, max_len, scale | None, 4 tensors of the ledger) -> status
+// code or None
+PyObject* pages_observe(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    ARGS(11);
+    const at::Tensor* q = tensor_or_null(args[2]);
+    PagesCall c;
+    tq_pages_ledger ledger = {};
+    if (!q || q->dim() != 4 || !pages_call(c, args[0], args[1], args[3], args[4], args[5], q->size(0))) {
+        if (PyErr_Occurred()) return nullptr;
+        Py_RETURN_NONE;
+    }
+    const int64_t d = c.pages->head_dim, qh = q->size(2), window = q->size(1);
+    const double scale = args[6] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!on(*q, *c.status) || !q->is_contiguous() || q->size(3) != d || qh < 1 || qh > INT32_MAX || window < 1 || window > INT32_MAX ||
+        dtype_code(q->scalar_type()) != (int)c.pages->dtype || !ledger_of(ledger, c, args + 7))
+        Py_RETURN_NONE;
+    c.batch.held = ledger.held;
+    c.batch.seen = ledger.seen;
+    const c10::cuda::CUDAGuard guard(c.status->get_device());
+    size_t need = 0;
+    int rc = tq_pages_observe_scratch_bytes(c.pages, &c.batch, (int32_t)window, (int32_t)qh, &need);
+    if (rc != TQ_OK) return PyLong_FromLong(rc);
+    const at::Tensor scratch = bytes_like(*q, need);
+    rc = tq_pages_observe(c.pages, &c.batch, q->data_ptr(), (int32_t)window, (int32_t)qh, (float)scale, ledger.mass, ledger.max_tokens,
+                          scratch.data_ptr(), need, c.status->data_ptr<int32_t>(), stream_of(*q));
+    if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
+    return PyLong_FromLong(rc);
+    END_HANDLE_TH_ERRORS
 }
 
 // pages_evict(pages, status, tables, lens, max_len, budget, recent, 4 tensors of the ledger, 4 of the one to write) -> new lengths,

@@ -30,6 +30,7 @@ struct Batch {
     const int32_t* table;
     const int32_t* lens;
     int table_stride, batch, max_seq_len;
+    const int32_t *held, *seen;    // of a ledger, or NULL
 };
 
 // Longest table index a length may reach is checked on the host (max_seq_len against the table's width); a length outside
@@ -100,13 +101,13 @@ inline Pages pages_of(const tq_pages* g) {
 constexpr int64_t MAX_UNITS = ((int64_t)1 << 31) - (1 << 20);
 // A table row covers max_seq_len tokens.
 inline int batch_check(const tq_pages* g, const tq_pages_batch* q) {
-    if (!q || !q->block_tables || !q->seq_lens) return TQ_ERR_NULL;
+    if (!q || !q->block_tables || !q->seq_lens || !q->held != !q->seen) return TQ_ERR_NULL;
     if (q->batch < 1 || q->max_seq_len < 1 || q->table_width < 1 || q->table_stride < q->table_width) return TQ_ERR_SHAPE;
     if ((int64_t)q->table_width * g->block_size < q->max_seq_len || q->max_seq_len > (1 << 30)) return TQ_ERR_RANGE;
     return TQ_OK;
 }
 inline Batch batch_of(const tq_pages_batch* q) {
-    return Batch{q->block_tables, q->seq_lens, q->table_stride, q->batch, q->max_seq_len};
+    return Batch{q->block_tables, q->seq_lens, q->table_stride, q->batch, q->max_seq_len, q->held, q->seen};
 }
 
 }  // namespace tqpg

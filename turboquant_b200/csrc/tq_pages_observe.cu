@@ -174,9 +174,16 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
     int done = 0;
     int b = n_tiles > 0 ? s_at[0] : 0, base_first = n_tiles > 0 ? s_at[2] : 0;     // base_first: where sequence b begins in the first launch's list
     int list = 0, tile0 = 0, n = 0, tiles = 0;
-    if (n_tiles > 0) {
+    int ordered = 0;                                                               // the slot from which on slots are in the sequence's order
+    auto begin = [&]() {                                                           // sequence b
         n = fresh_len(p.q, b, p.status);
         tiles = (n + OB_TILE - 1) / OB_TILE;
+        const int held = p.q.held != nullptr ? __ldcg(p.q.held + b) : 0;
+        ordered = held > 0 && __ldcg(p.q.seen + b) != held ? held : 0;
+        if (ordered > max(0, n - p.window) && tid == 0 && n > 0) atomicCAS(p.status, 0, (int)TQ_ERR_RANGE);
+    };
+    if (n_tiles > 0) {
+        begin();
         const int rel = lo - s_at[1];
         list = rel / tiles;
         tile0 = rel - list * tiles;
@@ -273,7 +280,7 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
             }
             // first launch: the last token that this thread's row sees
             const int my_row = twice ? lane_row & 63 : lane_row;
-            const int last = SECOND ? 0 : n - p.window + p.by_group.quotient(rt * OB_TILE + my_row);
+            const int at = SECOND ? 0 : n - p.window + p.by_group.quotient(rt * OB_TILE + my_row), last = at < ordered ? -1 : at;
             float m = -INFINITY, l = 0.f;
             bool bad = false;
 #pragma unroll 1
@@ -361,8 +368,8 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
                     }
                 } else {
                     const int t = t0 + lane_row;
-                    // query i sees token t from i = t - (n - window) on
-                    const int from = max(0, (t - n + p.window)) * p.by_group.d - rt * OB_TILE;
+                    // query i sees token t from i = t - (n - window) on, if it lies in the part that is in order
+                    const int from = min(max(0, max(t, ordered) - n + p.window), p.window) * p.by_group.d - rt * OB_TILE;
                     const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2);
                     uint64_t sum2[2] = {0ull, 0ull};
                     float sum = 0.f;
@@ -412,8 +419,7 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
             do {
                 base_first += tiles * per_seq_first;
                 ++b;
-                n = fresh_len(p.q, b, p.status);
-                tiles = (n + OB_TILE - 1) / OB_TILE;
+                begin();
             } while (n == 0 && b + 1 < p.q.batch);                                 // a share ends with its last tile: there is one ahead
         }
     }

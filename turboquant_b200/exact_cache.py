@@ -257,10 +257,11 @@ class PagedKVCache:
                 ledger: AttentionLedger, scale: Optional[float] = None) -> None:
         """Add to the ledger what the last `window` queries of every sequence give to its cached tokens: query (B, window, Qh,
         D), query i of a sequence of n tokens at position n - window + i, where it sees the tokens up to its own; a query before
-        the first token gives nothing.  For a cache that nothing has been evicted from (slots in the sequence's order)."""
+        the first token gives nothing.  In a sequence that tokens have been evicted from, the window is one of the tokens that came
+        after that (its slots are in order): a query further back gives nothing, and `status` reports it."""
         self._ledger(ledger, 0, 0)
         args = (self.addr, self._status)
-        rc = E.host().pages_observe(*args, query, block_tables, seq_lens, max_seq_len, scale, ledger.mass)
+        rc = E.host().pages_observe(*args, query, block_tables, seq_lens, max_seq_len, scale, *ledger._tensors)
         if rc is None:
             self._on_device(query=query)
             if query.dtype != self.spec.dtype:
@@ -272,7 +273,7 @@ class PagedKVCache:
             self._ledger(ledger, b, max_seq_len)
             if b == 0 or query.shape[1] == 0 or max_seq_len == 0:
                 return
-            rc = E.host().pages_observe(*args, self._rows(query), block_tables, seq_lens, max_seq_len, scale, ledger.mass)
+            rc = E.host().pages_observe(*args, self._rows(query), block_tables, seq_lens, max_seq_len, scale, *ledger._tensors)
         E.check(_lib.TQ_ERR_SHAPE if rc is None else rc, "tq_pages_observe")
 
     def evict(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int, ledger: AttentionLedger, budget: int,
