@@ -142,3 +142,25 @@ def test_observing_after_an_eviction_with_many_rows():
         _, p = O.attention(q[0].double().view(W, H, G, D), k[0].double(), v[0].double(), last=last)
         add, rel = p.sum((0, 2)), score_error(q.double(), k.double(), D ** -0.5)
         assert ((led.mass[0].cpu().double() - add).abs() <= add * (rel + (W * G + W * G // 128 + 2) * 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("W,G", [(4, 4), (40, 4), (1, 1)])
+def test_a_key_that_is_not_a_number(W, G):
+    """Every weight of a query that sees it is NaN, in whatever part of the sequence it lies; other sequences and rows are not touched."""
+    H, D, n = 2, 128, 5000
+    g = torch.Generator().manual_seed(W)
+    k, v = torch.randn(3, n, H, D, generator=g).to(BF16), torch.randn(3, n, H, D, generator=g).to(BF16)
+    k[0, 1024:1152, 1] = math.nan             # a tile of the product
+    k[1, 4000, 0, 7] = math.nan
+    cache, table, lens = cache_over(k, v, 16)
+    q = torch.randn(3, W, H * G, D, generator=g).to(BF16)
+    seen, step = AttentionLedger(3, H, n, "cuda"), AttentionLedger(3, H, n, "cuda")
+    cache.observe(q.cuda(), table, lens, n, seen)
+    out = cache.decode(q[:, -1].cuda(), table, lens, n, ledger=step).cpu().view(3, H, G, D)
+    whole = torch.tensor([[0, 1], [1, 0], [0, 0]], dtype=torch.bool)
+    for mass in (seen.mass.cpu(), step.mass.cpu()):
+        nan = torch.isnan(mass)
+        nan[:, :, n - W:] |= whole[..., None]      # a window's own tokens: not all queries see them, the last one does
+        assert torch.equal(nan.all(-1), whole) and torch.equal(nan.any(-1), whole)
+    assert torch.equal(torch.isnan(out).all(-1).all(-1), whole) and torch.equal(torch.isnan(out).any(-1).any(-1), whole)
+    assert cache.status() == 0

@@ -69,6 +69,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
+// 2^(x - top) of a piece's maximum x, 1 where it is the largest: sums that are NaN under a maximum of -inf (scores that are all NaN) stay NaN
+__device__ __forceinline__ float share_of_top(float x, float top) { return x == top ? 1.f : ex2(x - top); }
+
 // A length as it lies in the second-level cache: the second launch asks before it waits for the first one, which has waited for
 // everything ahead of it.
 __device__ __forceinline__ int fresh_len(const Batch& q, int b, int32_t* status) {
@@ -263,18 +266,17 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
                     float mx = m;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) mx = fmaxf(mx, v[k].x);
-                    if (mx == -INFINITY) continue;
-                    l *= ex2(m - mx);
+                    l *= share_of_top(m, mx);
                     m = mx;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) l = fmaf(v[k].y, ex2(v[k].x - mx), l);
+                    for (int k = 0; k < 8; ++k) l = fmaf(v[k].y, share_of_top(v[k].x, mx), l);
                 }
                 s_stat[tid] = make_float2(m, l);
                 __syncthreads();
                 if (tid < OB_TILE) {
                     const float2 o = s_stat[tid + OB_TILE];
                     const float mx = fmaxf(m, o.x);
-                    const float sum = mx == -INFINITY ? 0.f : l * ex2(m - mx) + o.y * ex2(o.x - mx);
+                    const float sum = l * share_of_top(m, mx) + o.y * share_of_top(o.x, mx);
                     s_lse[tid] = sum == 0.f || tid >= rows ? INFINITY : mx + log2f(sum);
                 }
             }
@@ -405,8 +407,7 @@ __global__ void __launch_bounds__(OB_THREADS, D == 256 ? 1 : 2) tq_pages_observe
                 if (tid < (twice ? 64 : OB_TILE)) {
                     float mx = m, sum = 0.f;
                     for (int k = tid; k < OB_THREADS; k += twice ? 64 : OB_TILE) mx = fmaxf(mx, s_stat[k].x);
-                    if (mx != -INFINITY)
-                        for (int k = tid; k < OB_THREADS; k += twice ? 64 : OB_TILE) sum = fmaf(s_stat[k].y, ex2(s_stat[k].x - mx), sum);
+                    for (int k = tid; k < OB_THREADS; k += twice ? 64 : OB_TILE) sum = fmaf(s_stat[k].y, share_of_top(s_stat[k].x, mx), sum);
                     p.stats[(((int64_t)(b * p.g.H + h) * p.row_tiles + rt) + blockIdx.x) * OB_TILE + tid] = make_float2(mx, sum);
                 }
             }
