@@ -523,6 +523,8 @@ int tq_pages_write(const tq_pages* pages, const void* key, const void* value, in
 /* Bytes of the tickets of tq_pages_decode and tq_pages_observe: zeroed once, zero again after every call.  Calls that may run at
  * the same time need tickets (and scratch, of any content) of their own. */
 size_t tq_pages_ticket_bytes(void);
+/* Without a ledger some 3 to 24 MB by head_dim and query heads a kv head; with_mass the scores beside it, 4 bytes a query head
+ * and token of max_seq_len, for as many sequences as 512 MB hold, one at least: a larger batch goes through in slices. */
 int tq_pages_decode_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t num_q_heads, int32_t with_mass, size_t* out);
 
 /* Attention of one new token per sequence, already in the pages as the last of its seq_lens tokens: query and out

@@ -164,3 +164,34 @@ def test_a_key_that_is_not_a_number(W, G):
         assert torch.equal(nan.all(-1), whole) and torch.equal(nan.any(-1), whole)
     assert torch.equal(torch.isnan(out).all(-1).all(-1), whole) and torch.equal(torch.isnan(out).any(-1).any(-1), whole)
     assert cache.status() == 0
+
+
+def test_a_ledgers_scratch_memory_is_bounded():
+    """Lengths of a few hundred under a bound of 2^20 tokens, as a captured step has it: 64 query heads would keep 268 MB of scores a
+    sequence.  The batch goes through in slices; a slice may be one sequence, and sequences may be empty."""
+    H, G, D, most = 2, 32, 64, 2 ** 20
+    g = torch.Generator().manual_seed(11)
+    k, v = torch.randn(7, 700, H, D, generator=g).to(BF16), torch.randn(7, 700, H, D, generator=g).to(BF16)
+    cache, table, _ = cache_over(k, v, 16)
+    wide = torch.full((7, most // 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    n = [500, 0, 33, 1, 700, 16, 257]
+    lens = torch.tensor(n, dtype=torch.int32, device="cuda")
+    q = torch.randn(7, H * G, D, generator=g).to(BF16)
+    led = AttentionLedger(7, H, most, "cuda")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = cache.decode(q.cuda(), wide, lens, most, ledger=led)
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 29 + 2 ** 26
+    assert cache.status() == 0
+    for b, m in enumerate(n):
+        rows = k[b, :m].double(), v[b, :m].double()
+        qb = q[b].double().view(1, H, G, D)
+        ref, p = O.attention(qb, *rows)
+        add, rel = p[0].sum(1), score_error(qb, k.double(), D ** -0.5)
+        assert ((led.mass[b, :, :m].cpu().double() - add).abs() <= add * (rel + (G + 1) * 2.0 ** -24)).all() and not led.mass[b, :, m:].any()
+        size = torch.einsum("rhgn,nhd->rhgd", p, rows[1].abs())
+        bound = ref.abs() * torch.finfo(BF16).eps / 2 * (1 + 2.0 ** -6) + size * (rel + 2.0 ** -18 + (m / 8 + 2) * 2.0 ** -22)
+        assert ((out[b].cpu().double().view(1, H, G, D) - ref).abs() <= bound).all()

@@ -15,3 +15,21 @@ def test_what_a_ledger_holds_comes_in_a_pair(lib, call):  # noqa: F811
     assert ask() == 0
     call.batch.held = None
     assert ask() == NULL
+
+
+def test_scratch_of_a_ledger_is_bounded(lib, call):  # noqa: F811
+    """What the scores take beside the rest: 4 bytes a query head and token of the bound, 512 MB or one sequence at most."""
+    def scores(batch, tokens, heads=64):
+        call.batch.batch, call.batch.max_seq_len, call.batch.table_width, call.batch.table_stride = batch, tokens, 1 << 26, 1 << 26
+        got = []
+        for mass in (0, 1):
+            size = C.c_size_t(0)
+            assert lib.tq_pages_decode_scratch_bytes(C.byref(call.pages), C.byref(call.batch), heads, mass, C.byref(size)) == 0
+            got.append(size.value)
+        return got[1] - got[0]
+    sums = lambda rows: (rows * 64 * 4 + 255) // 256 * 256  # noqa: E731
+    assert scores(4, 1000) == 4 * 64 * 1008 * 4 + sums(4)
+    assert scores(16, 131072) == 2 ** 29 + sums(16)
+    for batch in (17, 64, 256):
+        assert scores(batch, 131072) == 2 ** 29 + sums(16)
+    assert scores(3, 1 << 22) == 2 ** 30 + sums(1) and scores(1000, 100000) == 20 * 64 * 100000 * 4 + sums(20)

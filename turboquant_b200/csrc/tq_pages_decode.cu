@@ -26,6 +26,8 @@
 // largest weight (a sink) makes the small weights all of the output: so fp16 weights are multiplied by 2^15 before they are
 // split, and the factor is taken off again with the division by the sum.  What is lost of a weight is then at most 2^-40 of the largest
 // one of the warp's share: up to 32768 values of size one, no more than half of the smallest step of an fp16 output.
+#include <algorithm>
+
 #include "tq_pages.cuh"
 
 using namespace tqpg;
@@ -704,43 +706,54 @@ __global__ void __launch_bounds__(256) tq_pages_ledger_kernel(const Batch q, con
                                                               int32_t* status) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int b = blockIdx.x / H, t0 = blockIdx.y * 256 * LEDGER_TOK + threadIdx.x;
+    const int b = blockIdx.x / H;
     const int n = seq_len(q, b, status);
     const int64_t row = (int64_t)blockIdx.x * G;
     float* to = mass + blockIdx.x * mass_stride;
-    float sum[LEDGER_TOK], old[LEDGER_TOK];
+    for (int tile = blockIdx.y * 256 * LEDGER_TOK; tile < n; tile += gridDim.y * 256 * LEDGER_TOK) {
+        const int t0 = tile + threadIdx.x;
+        float sum[LEDGER_TOK], old[LEDGER_TOK];
 #pragma unroll
-    for (int k = 0; k < LEDGER_TOK; ++k) {
-        sum[k] = 0.f;
-        if (t0 + k * 256 < n) old[k] = to[t0 + k * 256];
-    }
+        for (int k = 0; k < LEDGER_TOK; ++k) {
+            sum[k] = 0.f;
+            if (t0 + k * 256 < n) old[k] = to[t0 + k * 256];
+        }
 #pragma unroll 4
-    for (int i = 0; i < G; ++i) {
-        const float* s = scores + (row + i) * score_stride + t0;
-        const float base = lse[row + i];
+        for (int i = 0; i < G; ++i) {
+            const float* s = scores + (row + i) * score_stride + t0;
+            const float base = lse[row + i];
+#pragma unroll
+            for (int k = 0; k < LEDGER_TOK; ++k)
+                if (t0 + k * 256 < n) sum[k] += ex2(__ldcs(s + k * 256) - base);
+        }
 #pragma unroll
         for (int k = 0; k < LEDGER_TOK; ++k)
-            if (t0 + k * 256 < n) sum[k] += ex2(__ldcs(s + k * 256) - base);
+            if (t0 + k * 256 < n) to[t0 + k * 256] = old[k] + sum[k];
     }
-#pragma unroll
-    for (int k = 0; k < LEDGER_TOK; ++k)
-        if (t0 + k * 256 < n) to[t0 + k * 256] = old[k] + sum[k];
 }
 
+// The scores of a ledger's call take 4 bytes a query head and token of the host's bound, whatever the lengths are.  Beyond
+// SCORES_MOST the batch goes through in slices of sequences, one at least, over the same scratch memory: 256 sequences of 300 to
+// 600 tokens, 64 query heads, under a bound of 131072 take 0.5 GB in the place of 8.6 and 365 us in 17 slices; 64 of them 90 us in
+// five.
+constexpr size_t SCORES_MOST = (size_t)512 << 20;
 struct Scratch {
     size_t partials, lse, scores, bytes;
     int64_t score_stride;
+    int slice;                // sequences at a time
 };
 int row_tiles(int G) { return (G + 15) / 16; }
 Scratch scratch_of(const tq_pages* g, const tq_pages_batch* q, int Qh, bool ledger) {
     const int nt = Qh / g->num_kv_heads > 8 ? 2 : 1;
     const size_t slot = (size_t)g->head_dim / 16 * nt * 128 + nt * 16;      // Shape<>::SLOT, Shape<>::NW warps
     Scratch s;
+    s.score_stride = ((int64_t)q->max_seq_len + 15) / 16 * 16;
+    const size_t each = (size_t)Qh * s.score_stride * 4;
+    s.slice = !ledger || each * q->batch <= SCORES_MOST ? q->batch : each >= SCORES_MOST ? 1 : (int)(SCORES_MOST / each);
     s.partials = 0;
     s.lse = (size_t)tq_sm_count() * (2 + 8) * slot * 4;
-    s.score_stride = ((int64_t)q->max_seq_len + 15) / 16 * 16;
-    s.scores = s.lse + (ledger ? ((size_t)q->batch * Qh * 4 + 255) / 256 * 256 : 0);
-    s.bytes = s.scores + (ledger ? (size_t)q->batch * Qh * s.score_stride * 4 : 0);
+    s.scores = s.lse + (ledger ? ((size_t)s.slice * Qh * 4 + 255) / 256 * 256 : 0);
+    s.bytes = s.scores + (ledger ? s.slice * each : 0);
     return s;
 }
 
@@ -787,7 +800,6 @@ extern "C" int tq_pages_decode(const tq_pages* pages, const tq_pages_batch* batc
     if (!query || !out || !scratch || !tickets || !status) return TQ_ERR_NULL;
     if (((uintptr_t)query & 15) || ((uintptr_t)out & 15) || ((uintptr_t)scratch & 15)) return TQ_ERR_ALIGN;
     if (mass && mass_stride < batch->max_seq_len) return TQ_ERR_RANGE;
-    if (mass && batch->max_seq_len > 65535 * 256 * LEDGER_TOK) return TQ_ERR_SHAPE;      // a grid's second dimension
     const Scratch s = scratch_of(pages, batch, num_q_heads, mass != nullptr);
     if (scratch_bytes < s.bytes) return TQ_ERR_WORKSPACE;
     DecodeParams p;
@@ -809,14 +821,28 @@ extern "C" int tq_pages_decode(const tq_pages* pages, const tq_pages_batch* batc
     cudaStream_t st = (cudaStream_t)stream;
     const int sms = tq_sm_count(), ctas = sms < MAX_CTAS ? sms : MAX_CTAS, two = p.G > 8;
     tq_note_launch(st, TQ_LAUNCH_WAITED);
-    switch (pages->head_dim) {
-        case 64: rc = two ? launch_dtype<64, 2>(p, pages->dtype, ctas, st) : launch_dtype<64, 1>(p, pages->dtype, ctas, st); break;
-        case 128: rc = two ? launch_dtype<128, 2>(p, pages->dtype, ctas, st) : launch_dtype<128, 1>(p, pages->dtype, ctas, st); break;
-        default: rc = two ? launch_dtype<256, 2>(p, pages->dtype, ctas, st) : launch_dtype<256, 1>(p, pages->dtype, ctas, st); break;
-    }
-    if (rc != TQ_OK || !mass) return rc;
     const int tile = 256 * LEDGER_TOK;
-    const dim3 grid((unsigned)(batch->batch * pages->num_kv_heads), (unsigned)((batch->max_seq_len + tile - 1) / tile));
-    return launch_behind(tq_pages_ledger_kernel, grid, 256, 0, st, p.q, (const float*)p.scores, p.score_stride, (const float*)p.lse,
-                         (int)pages->num_kv_heads, p.G, mass, mass_stride, status);
+    const int64_t rows = (int64_t)s.slice * num_q_heads * pages->head_dim * 2;      // bytes of a slice's queries and outputs
+    for (int b = 0; b < batch->batch; b += s.slice) {
+        p.q.batch = batch->batch - b < s.slice ? batch->batch - b : s.slice;
+        switch (pages->head_dim) {
+            case 64: rc = two ? launch_dtype<64, 2>(p, pages->dtype, ctas, st) : launch_dtype<64, 1>(p, pages->dtype, ctas, st); break;
+            case 128: rc = two ? launch_dtype<128, 2>(p, pages->dtype, ctas, st) : launch_dtype<128, 1>(p, pages->dtype, ctas, st); break;
+            default: rc = two ? launch_dtype<256, 2>(p, pages->dtype, ctas, st) : launch_dtype<256, 1>(p, pages->dtype, ctas, st); break;
+        }
+        if (rc != TQ_OK || !mass) return rc;
+        // four waves of CTAs, not one for every tile that the bound allows: 512 rows under a bound of 131072 tokens are 65536 of those
+        const int64_t heads = (int64_t)p.q.batch * pages->num_kv_heads, tiles = ((int64_t)batch->max_seq_len + tile - 1) / tile;
+        const int64_t most = std::max<int64_t>(1, 4 * 8 * sms / heads);
+        const dim3 grid((unsigned)heads, (unsigned)std::min(tiles, most));
+        rc = launch_behind(tq_pages_ledger_kernel, grid, 256, 0, st, p.q, (const float*)p.scores, p.score_stride, (const float*)p.lse,
+                           (int)pages->num_kv_heads, p.G, mass, mass_stride, status);
+        if (rc != TQ_OK) return rc;
+        p.q.table += (int64_t)s.slice * p.q.table_stride;
+        p.q.lens += s.slice;
+        p.query += rows;
+        p.out += rows;
+        mass += (int64_t)s.slice * pages->num_kv_heads * mass_stride;
+    }
+    return TQ_OK;
 }

@@ -224,7 +224,8 @@ class PagedKVCache:
         """One decode token per sequence, already written as the last of its `seq_lens` tokens: query (B, Qh, D),
         block_tables (B, max_blocks) int32, seq_lens (B,) int32 -> (B, Qh, D); an empty sequence's rows are zero.  Every
         sequence of the step in one launch.  With a ledger the weight every cached token received, summed over the query heads
-        of its kv head, is added to the ledger's mass."""
+        of its kv head, is added to the ledger's mass; the call then takes 4 bytes a query head and token of `max_seq_len` for as
+        many sequences as 512 MB hold (one at least), and a larger batch goes through in slices of that many."""
         if ledger is not None:
             self._ledger(ledger, 0, 0)
         args = (self.addr, self._status, self._tickets)
