@@ -195,3 +195,30 @@ def test_a_ledgers_scratch_memory_is_bounded():
         size = torch.einsum("rhgn,nhd->rhgd", p, rows[1].abs())
         bound = ref.abs() * torch.finfo(BF16).eps / 2 * (1 + 2.0 ** -6) + size * (rel + 2.0 ** -18 + (m / 8 + 2) * 2.0 ** -22)
         assert ((out[b].cpu().double().view(1, H, G, D) - ref).abs() <= bound).all()
+
+
+def test_tensors_with_a_dimension_of_one():
+    """One token of padded rows, one kv head, one page, one sequence's table as a column: torch lets such a dimension have any
+    stride, and calls the tensor contiguous."""
+    g = torch.Generator().manual_seed(3)
+    odd = torch.randn(5, 260, generator=g).to(BF16).cuda()
+    rows = odd[:, :256].unflatten(1, (2, 128))                    # (5, 2, 128), strides (260, 128, 1)
+    cache = PagedKVCache.allocate(ExactCacheSpec(128, 2), 3, "cuda")
+    for t in (1, 2, 5):
+        slots = torch.arange(t, device="cuda") + 7 * t
+        cache.write(rows[:t], rows[:t].flip(1), slots)
+        flat = cache.key_cache.flatten(0, 1)[slots], cache.value_cache.flatten(0, 1)[slots]
+        assert torch.equal(flat[0], rows[:t]) and torch.equal(flat[1], rows[:t].flip(1))
+    planes = torch.zeros(4099, dtype=BF16, device="cuda")[:4096].as_strided((2, 16, 1, 128), (2048, 128, 1, 1))
+    single = PagedKVCache(ExactCacheSpec(128, 1), planes, torch.zeros_like(planes))
+    one = torch.randn(3, 129, generator=g).to(BF16).cuda().as_strided((3, 1, 128), (128, 131, 1))
+    single.write(one, one, torch.tensor([4, 30, 9], device="cuda"))
+    assert torch.equal(planes.flatten(0, 1)[[4, 30, 9]], one)
+    lens = torch.tensor([9], dtype=torch.int32, device="cuda")
+    column = torch.tensor([[1, 5], [7, 7]], dtype=torch.int32, device="cuda").t()[:1, :1]      # (1, 1), strides (1, 2)
+    q = torch.randn(1, 4, 128, generator=g).to(BF16).cuda()
+    plain = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    assert column.stride(1) != 1 and torch.equal(single.decode(q, column, lens, 16), single.decode(q, plain, lens, 16))
+    led = AttentionLedger(1, 1, 16, "cuda")
+    single.observe(q[:, None], column, lens, 16, led)
+    assert single.evict(column, lens, 16, led, 5).tolist() == [5] and single.status() == 0 and cache.status() == 0

@@ -2,7 +2,11 @@
 
 import ctypes as C
 
+import pytest
+import torch
+
 from tests.test_pages_cpu import NULL, cache, call, lib  # noqa: F401  fixtures
+from turboquant_b200 import ExactCacheSpec, PagedKVCache
 
 
 def test_what_a_ledger_holds_comes_in_a_pair(lib, call):  # noqa: F811
@@ -33,3 +37,22 @@ def test_scratch_of_a_ledger_is_bounded(lib, call):  # noqa: F811
     for batch in (17, 64, 256):
         assert scores(batch, 131072) == 2 ** 29 + sums(16)
     assert scores(3, 1 << 22) == 2 ** 30 + sums(1) and scores(1000, 100000) == 20 * 64 * 100000 * 4 + sums(20)
+
+
+def test_planes_with_a_dimension_of_one(cache):  # noqa: F811
+    """The stride of a dimension of one, odd or different between the planes, is nobody's business; that of a larger one is."""
+    bf = torch.bfloat16
+    odd = lambda shape, strides: torch.zeros(8192, dtype=bf).as_strided(shape, strides)  # noqa: E731
+    for shape, a, b in (((1, 2, 2, 64), (777, 128, 64, 1), (1030, 128, 64, 1)), ((2, 1, 2, 64), (1024, 3, 64, 1), (1024, 64, 64, 1)),
+                        ((2, 2, 1, 64), (512, 64, 100, 1), (512, 64, 64, 1)), ((1, 1, 1, 64), (1, 3, 5, 1), (64, 64, 64, 1))):
+        spec = ExactCacheSpec(64, shape[2], block_size=shape[1])
+        made = PagedKVCache(spec, odd(shape, a), odd(shape, b)).c
+        for n, got, want in zip(shape, (made.stride_block, made.stride_token, made.stride_head), a):
+            assert got == (want if n > 1 else 0)
+    spec = ExactCacheSpec(64, 2, block_size=2)
+    with pytest.raises(ValueError):
+        PagedKVCache(spec, odd((2, 2, 2, 64), (516, 128, 64, 1)), odd((2, 2, 2, 64), (516, 128, 64, 1)))
+    with pytest.raises(ValueError):
+        PagedKVCache(spec, odd((2, 2, 2, 64), (512, 128, 64, 1)), odd((2, 2, 2, 64), (256, 128, 64, 1)))
+    with pytest.raises(ValueError):
+        PagedKVCache(spec, odd((1, 2, 2, 64), (512, 128, 64, 1)), odd((1, 2, 2, 64), (512, 256, 128, 2)))

@@ -523,6 +523,8 @@ struct PagesCall {
     const at::Tensor* status = nullptr;
     tq_pages_batch batch = {};
 };
+// of a dimension of one, which torch lets have any stride, 0
+inline int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 inline bool on(const at::Tensor& t, const at::Tensor& like) { return t.is_cuda() && t.get_device() == like.get_device(); }
 // pages, status, block tables, lengths and their bound; false: not as the kernels take them
 bool pages_call(PagesCall& c, PyObject* pages, PyObject* status, PyObject* tables, PyObject* lens, PyObject* max_len, int64_t batch) {
@@ -531,8 +533,8 @@ bool pages_call(PagesCall& c, PyObject* pages, PyObject* status, PyObject* table
     const at::Tensor *t = tensor_or_null(tables), *n = tensor_or_null(lens);
     const int64_t longest = PyLong_AsLongLong(max_len);
     if (PyErr_Occurred() || !c.status || !t || !n || longest < 1 || longest > INT32_MAX || batch < 1 || batch > INT32_MAX) return false;
-    if (!on(*t, *c.status) || !on(*n, *c.status) || t->dim() != 2 || t->scalar_type() != at::kInt || t->stride(1) != 1 || t->size(0) < batch ||
-        t->size(1) < 1 || t->size(1) > INT32_MAX || (t->size(0) > 1 && t->stride(0) < t->size(1)) || t->stride(0) > INT32_MAX || n->dim() != 1 ||
+    if (!on(*t, *c.status) || !on(*n, *c.status) || t->dim() != 2 || t->scalar_type() != at::kInt || t->size(0) < batch || t->size(1) < 1 ||
+        t->size(1) > INT32_MAX || (t->size(1) > 1 && t->stride(1) != 1) || (t->size(0) > 1 && t->stride(0) < t->size(1)) || t->stride(0) > INT32_MAX || n->dim() != 1 ||
         n->scalar_type() != at::kInt || n->size(0) < batch || !n->is_contiguous() || t->size(1) * c.pages->block_size < longest)
         return false;
     c.batch.block_tables = t->data_ptr<int32_t>();
@@ -586,8 +588,8 @@ PyObject* pages_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         slots->size(0) < k->size(0) || !slots->is_contiguous() || k->size(0) < 1)
         Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(status->get_device());
-    const int rc = tq_pages_write(g, k->data_ptr(), v->data_ptr(), k->size(0), k->stride(0), k->stride(1), v->stride(0), v->stride(1),
-                                  slots->data_ptr<int64_t>(), status->data_ptr<int32_t>(), stream_of(*status));
+    const int rc = tq_pages_write(g, k->data_ptr(), v->data_ptr(), k->size(0), stride_of(*k, 0), stride_of(*k, 1), stride_of(*v, 0),
+                                  stride_of(*v, 1), slots->data_ptr<int64_t>(), status->data_ptr<int32_t>(), stream_of(*status));
     if (rc == TQ_ERR_ALIGN) Py_RETURN_NONE;
     return PyLong_FromLong(rc);
     END_HANDLE_TH_ERRORS

@@ -132,15 +132,17 @@ class PagedKVCache:
                 raise TypeError(f"{name} must be {spec.dtype} like the spec, not {t.dtype}")
             if t.dim() != 4 or tuple(t.shape[1:]) != (spec.block_size, spec.num_kv_heads, spec.head_dim) or t.shape[0] < 1:
                 raise ValueError(f"{name} must be (num_blocks, {spec.block_size}, {spec.num_kv_heads}, {spec.head_dim})")
-        if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride() or key_cache.device != value_cache.device:
+        # a dimension of one may have any stride
+        strides, of_value = ([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)] for t in (key_cache, value_cache))
+        if key_cache.shape != value_cache.shape or strides != of_value or key_cache.device != value_cache.device:
             raise ValueError("key_cache and value_cache must be of one layout on one device")
-        if key_cache.stride(3) != 1 or any(s % 8 or s < 0 for s in key_cache.stride()[:3]) or \
+        if key_cache.stride(3) != 1 or value_cache.stride(3) != 1 or any(s % 8 for s in strides) or \
                 any(t.data_ptr() % 16 for t in (key_cache, value_cache)):
             raise ValueError("rows of the planes must be contiguous and 16-byte aligned")
         self.spec, self.key_cache, self.value_cache = spec, key_cache, value_cache
         self.device = key_cache.device
         self.c = _lib.tq_pages(key_cache.data_ptr(), value_cache.data_ptr(), E.dtype_code(spec.dtype), spec.block_size,
-                               key_cache.shape[0], spec.num_kv_heads, spec.head_dim, *key_cache.stride()[:3])
+                               key_cache.shape[0], spec.num_kv_heads, spec.head_dim, *strides)
         self.addr = C.addressof(self.c)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._tickets: dict = {}        # by stream
@@ -181,7 +183,7 @@ class PagedKVCache:
             raise ValueError(f"max_seq_len {max_seq_len} is out of range")
         if block_tables.shape[1] * self.spec.block_size < max_seq_len:
             raise ValueError(f"block_tables of {block_tables.shape[1]} pages do not hold {max_seq_len} tokens")
-        if block_tables.stride(1) != 1 or (block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1]):
+        if (block_tables.shape[1] > 1 and block_tables.stride(1) != 1) or (block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1]):
             block_tables = block_tables.contiguous()
         return block_tables, seq_lens.contiguous()
 
