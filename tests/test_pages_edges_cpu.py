@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_pages_cpu import NULL, cache, call, lib  # noqa: F401  fixtures
-from turboquant_b200 import ExactCacheSpec, PagedKVCache
+from turboquant_b200 import AttentionLedger, ExactCacheSpec, PagedKVCache
 
 
 def test_what_a_ledger_holds_comes_in_a_pair(lib, call):  # noqa: F811
@@ -56,3 +56,18 @@ def test_planes_with_a_dimension_of_one(cache):  # noqa: F811
         PagedKVCache(spec, odd((2, 2, 2, 64), (512, 128, 64, 1)), odd((2, 2, 2, 64), (256, 128, 64, 1)))
     with pytest.raises(ValueError):
         PagedKVCache(spec, odd((1, 2, 2, 64), (512, 128, 64, 1)), odd((1, 2, 2, 64), (512, 256, 128, 2)))
+
+
+def test_a_ledger_is_what_its_attributes_are(cache):  # noqa: F811
+    """A tensor put in the place of another counts for every call, not for some."""
+    taken = []
+    cache.host.pages_decode = cache.host.pages_observe = cache.host.pages_evict = lambda *args: taken.append(args)
+    table, lens, q = torch.zeros(3, 4, dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.zeros(3, 8, 128, dtype=torch.bfloat16)
+    led = AttentionLedger(3, 2, 64, "cpu")
+    led.mass, led.held = led.mass.clone(), led.held.clone()
+    for call_it in (lambda: cache.decode(q, table, lens, 64, ledger=led), lambda: cache.observe(q[:, None], table, lens, 64, led),
+                    lambda: cache.evict(table, lens, 64, led, 8)):
+        with pytest.raises(RuntimeError):          # nothing native answers
+            call_it()
+        assert any(a is led.mass for a in taken[-1])
+    assert sum(a is led.held for a in taken[-1]) == 2          # evict: the ledger that is read and the one that is written

@@ -87,7 +87,10 @@ class AttentionLedger:
         if len({t.device for t in (mass, positions, held, seen)}) != 1:
             raise ValueError("the tensors of a ledger are on one device")
         self.mass, self.positions, self.held, self.seen = mass, positions, held, seen
-        self._tensors = (mass, positions, held, seen)
+
+    @property
+    def _tensors(self):
+        return self.mass, self.positions, self.held, self.seen
 
     @classmethod
     def over(cls, mass: torch.Tensor, positions: torch.Tensor, held: torch.Tensor, seen: torch.Tensor) -> "AttentionLedger":
