@@ -222,3 +222,22 @@ def test_tensors_with_a_dimension_of_one():
     led = AttentionLedger(1, 1, 16, "cuda")
     single.observe(q[:, None], column, lens, 16, led)
     assert single.evict(column, lens, 16, led, 5).tolist() == [5] and single.status() == 0 and cache.status() == 0
+
+
+def test_a_bound_of_no_tokens():
+    """Lengths beyond it are clamped to nothing and reported by every call, and an empty table will do."""
+    k = torch.randn(3, 40, 2, 128, generator=torch.Generator().manual_seed(0)).to(BF16)
+    cache, table, lens = cache_over(k, k, 16)
+    q, none, empty = torch.ones(3, 8, 128, dtype=BF16, device="cuda"), torch.zeros_like(lens), table[:, :0]
+    before = cache.key_cache.clone()
+    for now, code in ((none, 0), (lens, RANGE), (torch.tensor([0, 0, -1], dtype=torch.int32, device="cuda"), RANGE)):
+        for t in (table, empty):
+            led = AttentionLedger(3, 2, 40, "cuda")
+            led.mass.fill_(2.0)
+            assert not cache.decode(q, t, now, 0, ledger=led).any() and cache.status() == code
+            cache.observe(q[:, None], t, now, 0, led)
+            assert cache.status() == code and (led.mass == 2.0).all()
+            assert cache.evict(t, now, 0, led, 5, 2).tolist() == [0, 0, 0] and cache.status() == code
+            assert not led.mass.any() and (led.positions == -1).all() and not led.held.any() and not led.seen.any()
+    assert torch.equal(cache.key_cache, before)
+    assert not cache.decode(q, empty, lens, 0, out=torch.ones_like(q)).any() and cache.status() == RANGE

@@ -14,7 +14,7 @@ from .build import HOST_PATH, LIB_PATH
 TQ_BLOCK_TOKENS = 16
 TQ_MAX_CENTROIDS = 16
 TQ_F32, TQ_BF16, TQ_F16 = 0, 1, 2
-TQ_ERR_SHAPE, TQ_ERR_ALIGN, TQ_ERR_UNSUPPORTED = -2, -3, -4
+TQ_ERR_SHAPE, TQ_ERR_ALIGN, TQ_ERR_UNSUPPORTED, TQ_ERR_RANGE = -2, -3, -4, -7
 
 
 class TQError(RuntimeError):

@@ -199,6 +199,12 @@ class PagedKVCache:
             raise ValueError(f"{name} of {tuple(ledger.mass.shape)} does not hold {batch} sequences of {self.spec.num_kv_heads} kv heads "
                              f"and {max_seq_len} tokens")
 
+    def _no_tokens(self, seq_lens: torch.Tensor) -> torch.Tensor:
+        """The lengths under a bound of no tokens at all: zeros; any other is out of range and reported, as a kernel would."""
+        wrong = (seq_lens != 0).any() & (self._status == 0)
+        self._status.masked_fill_(wrong, _lib.TQ_ERR_RANGE)
+        return torch.zeros_like(seq_lens)
+
     def _rows(self, t: torch.Tensor) -> torch.Tensor:
         """`t` as a contiguous tensor on a 16-byte boundary."""
         t = t.contiguous()
@@ -252,6 +258,8 @@ class PagedKVCache:
             block_tables, seq_lens = self._batch(b, block_tables, seq_lens, max_seq_len)
             if ledger is not None:
                 self._ledger(ledger, b, max_seq_len)
+            if b > 0 and max_seq_len == 0:
+                self._no_tokens(seq_lens[:b])
             if b == 0 or max_seq_len == 0:
                 return torch.zeros_like(query, memory_format=torch.contiguous_format) if out is None else out.zero_()
             res = E.host().pages_decode(*args, self._rows(query), block_tables, seq_lens, max_seq_len, scale, out, mass)
@@ -277,6 +285,8 @@ class PagedKVCache:
             b = query.shape[0]
             block_tables, seq_lens = self._batch(b, block_tables, seq_lens, max_seq_len)
             self._ledger(ledger, b, max_seq_len)
+            if b > 0 and max_seq_len == 0:
+                self._no_tokens(seq_lens[:b])
             if b == 0 or query.shape[1] == 0 or max_seq_len == 0:
                 return
             rc = E.host().pages_observe(*args, self._rows(query), block_tables, seq_lens, max_seq_len, scale, *ledger._tensors)
@@ -311,9 +321,9 @@ class PagedKVCache:
                 raise ValueError(f"budget {budget} is out of range")
             if b == 0:
                 return torch.zeros_like(seq_lens)
-            if max_seq_len == 0:
-                max_seq_len = 1                     # every sequence is empty: the ledgers still agree afterwards
-                tail = (max_seq_len, *tail[1:])
+            if max_seq_len == 0:                    # every sequence is empty: the ledgers still agree afterwards
+                tail = (1, *tail[1:])
+                seq_lens, block_tables = self._no_tokens(seq_lens), block_tables.new_zeros(b, 1)
             res = native(self.addr, self._status, block_tables, seq_lens, *tail)
             if type(res) is torch.Tensor:
                 return res
