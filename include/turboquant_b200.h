@@ -547,8 +547,8 @@ int tq_pages_observe(const tq_pages* pages, const tq_pages_batch* batch, const v
 /* Bring every sequence down to `budget` tokens, kv head by kv head.  Of n > budget tokens the `recent` latest by position stay,
  * then those with the largest mass (NaN above all numbers, ties: the lower slot).  Tokens kept in slots from `budget` on move,
  * in ascending order, into the free slots before it: rows, mass and position; rows from `budget` on stay as they are.  `out`
- * receives the ledger (mass 0 and position -1 behind the tokens that are left, up to max_tokens) and may be `ledger` itself;
- * new_lens (batch) the lengths.  Sequences do not share pages. */
+ * receives the ledger (mass 0 and position -1 behind the tokens that are left, up to max_tokens) and may be `ledger` itself, but
+ * not overlap it otherwise; new_lens (batch) the lengths.  Sequences do not share pages. */
 int tq_pages_evict_scratch_bytes(const tq_pages* pages, const tq_pages_batch* batch, int32_t budget, size_t* out);
 int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch, const tq_pages_ledger* ledger, const tq_pages_ledger* out,
                    int32_t budget, int32_t recent, int32_t* new_lens, void* scratch, size_t scratch_bytes, int32_t* status,

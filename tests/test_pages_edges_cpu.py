@@ -5,8 +5,8 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_pages_cpu import NULL, cache, call, lib  # noqa: F401  fixtures
-from turboquant_b200 import AttentionLedger, ExactCacheSpec, PagedKVCache
+from tests.test_pages_cpu import NULL, SHAPE, WORKSPACE, cache, call, lib  # noqa: F401  fixtures
+from turboquant_b200 import AttentionLedger, ExactCacheSpec, PagedKVCache, _lib
 
 
 def test_what_a_ledger_holds_comes_in_a_pair(lib, call):  # noqa: F811
@@ -71,3 +71,18 @@ def test_a_ledger_is_what_its_attributes_are(cache):  # noqa: F811
             call_it()
         assert any(a is led.mass for a in taken[-1])
     assert sum(a is led.held for a in taken[-1]) == 2          # evict: the ledger that is read and the one that is written
+
+
+@pytest.mark.parametrize("array", ["mass", "positions", "held", "seen"])
+def test_a_ledger_half_over_another_is_refused(lib, call, array):  # noqa: F811
+    base = call.base
+    evict = lambda out: lib.tq_pages_evict(C.byref(call.pages), C.byref(call.batch), C.byref(call.ledger), C.byref(out), 8, 2, base, base, 0,  # noqa: E731
+                                           base, None)
+    words = 3 if array in ("held", "seen") else 3 * 2 * 64
+    fields = dict(mass=base, positions=base, held=base, seen=base, max_tokens=64)
+    for shift, code in ((0, WORKSPACE), (4, SHAPE), (-4, SHAPE), ((words - 1) * 4, SHAPE), (words * 4, WORKSPACE), (-words * 4, WORKSPACE)):
+        assert evict(_lib.tq_pages_ledger(**{**fields, array: base + shift})) == code
+    wider = {**fields, "max_tokens": 65}
+    assert evict(_lib.tq_pages_ledger(**wider)) == SHAPE                # the same memory with rows of another length
+    apart = {**wider, "mass": base + 8 * 1024, "positions": base + 8 * 1024}
+    assert evict(_lib.tq_pages_ledger(**apart)) == WORKSPACE

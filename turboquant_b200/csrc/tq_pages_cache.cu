@@ -499,6 +499,11 @@ int evict_list(const tq_pages_batch* q, int budget) {      // moves of a row at 
     const int behind = q->max_seq_len - budget;
     return behind <= 0 ? 0 : behind < budget ? behind : budget;
 }
+// Two arrays that are neither the same nor apart: rows of one would be written before the other's are read.
+bool half_over(const void* a, int64_t a_words, const void* b, int64_t b_words) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return !(x == y && a_words == b_words) && x < y + b_words * 4 && y < x + a_words * 4;
+}
 int evict_check(const tq_pages* g, const tq_pages_batch* q, int budget) {
     int rc = pages_check(g);
     if (rc == TQ_OK) rc = batch_check(g, q);
@@ -553,9 +558,12 @@ extern "C" int tq_pages_evict(const tq_pages* pages, const tq_pages_batch* batch
         if (l->max_tokens < batch->max_seq_len) return TQ_ERR_RANGE;
     }
     if (recent < 0 || recent > budget) return TQ_ERR_SHAPE;
+    const int64_t rows = (int64_t)batch->batch * pages->num_kv_heads, words = rows * ledger->max_tokens, out_words = rows * out->max_tokens;
+    if (half_over(ledger->mass, words, out->mass, out_words) || half_over(ledger->positions, words, out->positions, out_words) ||
+        half_over(ledger->held, batch->batch, out->held, batch->batch) || half_over(ledger->seen, batch->batch, out->seen, batch->batch))
+        return TQ_ERR_SHAPE;
     if (scratch_bytes < need) return TQ_ERR_WORKSPACE;
     if ((uintptr_t)scratch & 15) return TQ_ERR_ALIGN;
-    const int64_t rows = (int64_t)batch->batch * pages->num_kv_heads;
     EvictParams p;
     p.g = pages_of(pages);
     p.q = batch_of(batch);

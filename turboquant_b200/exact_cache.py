@@ -299,9 +299,9 @@ class PagedKVCache:
         Of a sequence with more tokens the `recent` latest by position stay, then those with the largest mass (NaN above every
         number; of equal ones the lower slot).  Kept tokens in slots from `budget` on move, in ascending order, into the free
         slots before it, row, mass and position; the order of a cache's tokens means nothing to attention.  Pages behind
-        the new length are the engine's to take back.  The ledger is brought up to date in place, or written to `out`; slots
-        behind the new length have mass 0 and position -1 there.  `seq_lens` is left as it is.  Sequences must not share pages
-        (a common prefix would be rearranged for one under the other)."""
+        the new length are the engine's to take back.  The ledger is brought up to date in place, or written to `out` (itself or
+        another, not one half over it); slots behind the new length have mass 0 and position -1 there.  `seq_lens` is left as it
+        is.  Sequences must not share pages (a common prefix would be rearranged for one under the other)."""
         self._ledger(ledger, 0, 0)
         out = ledger if out is None else out
         self._ledger(out, 0, 0, "out")
