@@ -241,3 +241,22 @@ def test_a_bound_of_no_tokens():
             assert not led.mass.any() and (led.positions == -1).all() and not led.held.any() and not led.seen.any()
     assert torch.equal(cache.key_cache, before)
     assert not cache.decode(q, empty, lens, 0, out=torch.ones_like(q)).any() and cache.status() == RANGE
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_one_query_observed_adds_what_its_decode_adds(dtype):
+    """From no mass at all, every increment against the other's: two ways of adding the same products, each within its bound."""
+    H, G, D, n = 2, 4, 128, 900
+    g = torch.Generator().manual_seed(17)
+    k, v = torch.randn(3, n, H, D, generator=g).to(dtype), torch.randn(3, n, H, D, generator=g).to(dtype)
+    cache, table, lens = cache_over(k, v, 16)
+    lens[1], lens[2] = 77, 1
+    q = torch.randn(3, H * G, D, generator=g).to(dtype)
+    a, b = AttentionLedger(3, H, n, "cuda"), AttentionLedger(3, H, n, "cuda")
+    cache.decode(q.cuda(), table, lens, n, ledger=a)
+    cache.observe(q[:, None].cuda(), table, lens, n, b)
+    rel = score_error(q.double(), k.double(), D ** -0.5) + (G + 1) * 2.0 ** -24
+    a, b = a.mass.cpu().double(), b.mass.cpu().double()
+    assert ((a - b).abs() <= 2 * rel * torch.minimum(a, b) * (1 + 2.0 ** -6)).all()
+    assert (a[0] > 0).all() and (a[1, :, :77] > 0).all() and not a[1, :, 77:].any() and cache.status() == 0
+    assert ((a.sum(-1) - G).abs() <= G * rel).all()
