@@ -520,7 +520,7 @@ int tq_pages_write(const tq_pages* pages, const void* key, const void* value, in
                    int64_t key_stride_head, int64_t value_stride_token, int64_t value_stride_head, const int64_t* slot_mapping,
                    int32_t* status, void* stream);
 
-/* Bytes of the tickets of tq_pages_decode and tq_pages_observe: zeroed once, zero again after every call.  Calls that may run at
+/* Bytes of the tickets of tq_pages_decode: zeroed once, zero again after every call.  Calls that may run at
  * the same time need tickets (and scratch, of any content) of their own. */
 size_t tq_pages_ticket_bytes(void);
 /* Without a ledger some 3 to 24 MB by head_dim and query heads a kv head; with_mass the scores beside it, 4 bytes a query head

@@ -55,7 +55,9 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Launch as a programmatic dependent: the CTAs may take their places while the launch ahead finishes.  Every kernel launched so
-// waits for it before it reads or writes anything, and lets the launch behind begin only after that.
+// waits for it before it reads or writes anything, and lets the launch behind begin only after that, with one exception: the
+// second launch of an observation reads lengths, tables, queries and keys (and may note an error) before its wait.  It directly
+// follows the first one, which writes none of those and has waited for everything ahead before this one may begin.
 template <class... P, class... A>
 inline int launch_behind_as(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};

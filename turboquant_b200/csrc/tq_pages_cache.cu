@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(WR_THREADS) tq_pages_write_kernel(const WriteP
 // count a row and keep every list in ascending order.
 //
 // A token that moves goes into a list with its mass and position; the second launch, which needs the list for the rows, puts them in
-// their places (in this one a mover would have to wait for the holes of the other CTAs: 512 rows of 2112 21.0 us in the place of
-// 19.9, 32 of up to 32768 46.6 in the place of 45.0, one of 32768 28 in the place of 25).
+// their places (in this one a mover would have to wait for the holes of the other CTAs: 1.1 us more for 512 rows of 2112, 1.6 for
+// 32 of up to 32768, 2.7 for one of 32768).
 //
 // Bound by the chain of loads, exchanges and lists.  Both launches take 9.6 us for 300 slots, 19.3 for 512 rows of 2112, of which
 // moving the rows is 8 (four CTAs an SM at 56 registers; at 40 they spill and it is 16 longer), 43.5 for 32 rows of up to 32768 in

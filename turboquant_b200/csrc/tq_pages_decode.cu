@@ -1,8 +1,8 @@
 // Attention of one new token per sequence over the exact paged cache.
 //
 // For a kv head with its group of G query heads:  s_gt = scale <q_g, k_t>,  out_g = sum_t 2^(s'_gt - m) v_t / sum_t 2^(s'_gt - m)
-// with s' = s log2(e) and m a running maximum; keys and values are read once.  The bound is HBM: 4 D bytes a token and kv head
-// against 4 G D operations.
+// with s' = s log2(e) and m a running maximum; keys and values are read once for every sixteen query heads of a kv head.  The bound
+// is HBM: 4 D bytes a token and kv head against 4 G D operations.
 //
 // The batch is one list of UNITS (16 tokens of one kv head of one sequence) in the order sequence, head, token.  Every CTA
 // (one per SM) takes an equal share of the list and every warp an equal share of that, whatever the lengths are: a share may
@@ -14,7 +14,8 @@
 // one that spans CTAs through at most two partial results a CTA and a ticket, in the order of the list: the same launch gives
 // the same bits every time.
 //
-// Measured: 64 sequences of 1024 to 32768 tokens, 64 / 8 heads of 128, 3.9 GB: 574 us, 6.7 TB/s.  One sequence of 32768, 16 / 4
+// Measured: 64 sequences of 1024 to 32768 tokens, 64 / 8 heads of 128, 3.9 GB: 574 us, 6.7 TB/s (call after call: part
+// of it still lies in L2).  One sequence of 32768, 16 / 4
 // heads of 256, 134 MB: 39 us, of which 23 are streaming, 4 the way to the first keys (lengths, table, rows) and 10 the joins
 // (in the CTA 2.5, ticket 1.5, across CTAs 5: chains of loads in code that runs once).  A single short sequence: 7 us.
 //

@@ -2,8 +2,8 @@
 //
 // Rows r = (query i of the window, query head of the kv head's group), R = window * G of them:
 //     s_rt = scale <q_r, k_t>,  t <= n - window + i(r);   lse_r = log2 sum_t 2^(s_rt);   mass_t += sum_r 2^(s_rt - lse_r)
-// (s in the log2 domain).  lse needs every key before the first weight is known, so the keys are gone over twice: the first launch
-// keeps a running maximum and sum per row and split, the second forms the weights.  Both are products of 128 x 128 tiles on the
+// (s in the log2 domain).  lse needs every key before the first weight is known, so the keys are gone over twice (for every 128
+// rows): the first launch keeps a running maximum and sum per row and split, the second forms the weights.  Both are products of 128 x 128 tiles on the
 // 5th-generation tensor cores, turned so that what is summed lies in one thread: queries in the rows (tensor-memory lanes) of the
 // first, whose threads sum along the keys, tokens in the rows of the second, whose threads sum along the queries.
 //
@@ -12,8 +12,9 @@
 // of tile i - 1 run at the same time.  Key tiles lie in shared memory as the tensor cores want them (64 channels a box, 128-byte
 // swizzle), brought by 16-byte asynchronous copies through the block table, so that a page may end anywhere.
 //
-// Measured: 16 queries of 8 sequences of 4096 to 32768, 32 / 8 heads of 128: 154 us for two times 291 MB; copies alone take 54 us a
-// launch, products and exponentials alone 44, and both want the SM's shared memory.  32 queries of one prompt of 5003: 19 us.
+// Measured: 16 queries of 8 sequences of 4096 to 32768, 32 / 8 heads of 128: 156 us for two times 291 MB.  Copies alone take 54 us
+// a launch, products and exponentials alone 44; the rest is their hand-over (a barrier of the CTA for every tile, two in the second
+// launch; no unit is busy for half of the time).  32 queries of one prompt of 5003: 19 us.
 #include "tq_pages.cuh"
 #include "tq_tcgen05.cuh"
 

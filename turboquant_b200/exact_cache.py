@@ -162,7 +162,7 @@ class PagedKVCache:
 
     def status(self) -> int:
         """0, or the first device-side error since the last call (a `tq_status`: an index or a length out of range); reading
-        clears it.  Synchronises."""
+        clears it.  Waits for the current stream; calls on others are the caller's to wait for first."""
         code = int(self._status.item())
         if code:
             self._status.zero_()
