@@ -3,9 +3,10 @@
 // Rows r = (query i of the window, query head of the kv head's group), R = window * G of them:
 //     s_rt = scale <q_r, k_t>,  t <= n - window + i(r);   lse_r = log2 sum_t 2^(s_rt);   mass_t += sum_r 2^(s_rt - lse_r)
 // (s in the log2 domain).  lse needs every key before the first weight is known, so the keys are gone over twice (for every 128
-// rows): the first launch keeps a running maximum and sum per row and split, the second forms the weights.  Both are products of 128 x 128 tiles on the
-// 5th-generation tensor cores, turned so that what is summed lies in one thread: queries in the rows (tensor-memory lanes) of the
-// first, whose threads sum along the keys, tokens in the rows of the second, whose threads sum along the queries.
+// rows): the first launch keeps a running maximum and sum per row and split, the second forms the weights.  Both are products of
+// 128 x 128 tiles on the 5th-generation tensor cores, turned so that what is summed lies in one thread: queries in the rows
+// (tensor-memory lanes) of the first, whose threads sum along the keys, tokens in the rows of the second, whose threads sum along
+// the queries.
 //
 // The tiles (128 tokens of one kv head of one sequence) of a batch are one list in the order sequence, head, row tile, token, of
 // which every CTA, two an SM, takes an equal share.  In a share, copies of tile i + 1, the product of tile i and the exponentials
