@@ -15,8 +15,9 @@
 // the same bits every time.
 //
 // Measured: 64 sequences of 1024 to 32768 tokens, 64 / 8 heads of 128, 3.9 GB: 574 us, 6.7 TB/s (call after call:
-// part of it still lies in L2).  One sequence of 32768, 16 / 4 heads of 256, 134 MB: 39 us, of which 23 are streaming, 4 the way to the first keys (lengths, table, rows) and 10 the joins
-// (in the CTA 2.5, ticket 1.5, across CTAs 5: chains of loads in code that runs once).  A single short sequence: 7 us.
+// part of it still lies in L2).  One sequence of 32768, 16 / 4 heads of 256, 134 MB: 39 us, of which 23 are streaming, 4 the way to
+// the first keys (lengths, table, rows) and 10 the joins (in the CTA 2.5, ticket 1.5, across CTAs 5: chains of loads in code that
+// runs once).  A single short sequence: 7 us.
 //
 // Products: S^T = K Q^T and O^T = V^T P^T as m16n8k16, tokens resp. channels in the 16 rows, eight query heads in the columns,
 // so that a group of up to eight pads nothing else.  tcgen05 would want 128 rows of operands through shared memory for eight
